@@ -59,7 +59,7 @@ const char* vince_last_error(void);
 /* Bumped whenever an exported signature, a struct layout or a dtype code changes.  vince_abi_version() returns the value the library
  * was BUILT with; a binding compares it at load (vince_amd/_lib.py: a stale .so behind VINCE_HIP_LIB would otherwise be called with
  * shifted arguments). */
-#define VINCE_ABI_VERSION 12
+#define VINCE_ABI_VERSION 13
 int vince_abi_version(void);
 
 /* Measurement aid (bench.py): while enabled, every conv_igemm / conv_wgrad launch is bracketed by a hipEvent pair on
@@ -535,6 +535,22 @@ int vince_l2norm_bwd(const float* x, const float* norms, const float* dout, floa
                      float eps, void* stream);
 int vince_relu_bwd(const float* dout, const float* act, float* dx, int64_t n, void* stream);
 int vince_colsum(const float* x, float* out, int32_t rows, int32_t cols, void* stream); /* out[c] += sum_r x[r][c] */
+/* Layer norm over the last axis of x[rows][cols] (dtype VINCE_F32 or VINCE_BF16; parameters, statistics and their sums fp32): the
+ * per-sample normalisation a projection head can have between its two Linears (no reference call site: --head-norm layer).
+ *   _fwd: mean = sum x / cols;  rstd = 1 / sqrt(sum (x - mean)^2 / cols + eps);  out = (x - mean) rstd weight + bias, and with relu != 0
+ *     max(out, 0).  weight float[cols] and bias float[cols] may be NULL (1 and 0; no bias without a weight); mean, rstd float[rows].
+ *   _bwd: d = dout, or 0 where act is given and act <= 0 (the ReLU's output: what vince_relu_bwd tests); g = d weight;
+ *     xhat = (x - mean) rstd;  dx = rstd (g - avg(g) - xhat avg(g xhat)), averages over a row;
+ *     dweight = sum over the rows of d xhat, dbias = sum of d (accumulate != 0: added to what is there), fixed order of summation.
+ *     dweight and dbias may both be NULL.  scratch: vince_layer_norm_bwd_scratch_bytes(), not read before it is written.
+ * No alignment beyond the element's is needed, rows may be 0 (cols >= 1), a value that is not finite spoils its own row (and its
+ * columns' sums) only.  (ABI 13) */
+int vince_layer_norm_fwd(int dtype, const void* x, const float* weight, const float* bias, void* out, float* mean, float* rstd,
+                         int64_t rows, int32_t cols, float eps, int32_t relu, void* stream);
+size_t vince_layer_norm_bwd_scratch_bytes(int dtype, int64_t rows, int32_t cols);
+int vince_layer_norm_bwd(int dtype, const void* x, const float* weight, const float* mean, const float* rstd, const void* dout,
+                         const void* act, void* dx, float* dweight, float* dbias, int32_t accumulate, int64_t rows, int32_t cols,
+                         void* scratch, size_t scratch_bytes, void* stream);
 /* The reference asserts torch.isfinite(total_loss) on EVERY iteration (solvers/vince_solver.py:446-452), a host sync per step.
  * Here the check stays on the device: latch[0] += 1 and latch[1] = step + 1 (first offender only) when *value is NaN or +-inf.
  * The caller zeroes latch (int64[2]) once, enqueues this every step and reads the latch whenever it synchronises anyway. */
@@ -602,6 +618,31 @@ int vince_ema_flat(float* key, const float* query, int64_t n, float momentum, vo
  * d = g + wd*p; buf = buf*mom + d; p -= lr*buf.  grad_scale multiplies g first (1/world for DP mean). */
 int vince_sgd_flat(float* param, const float* grad, float* buf, int64_t n, float lr, float momentum,
                    float weight_decay, float grad_scale, void* stream);
+
+/* Global gradient norm over many tensors, and clipping (no reference call site: --max-grad-norm).  A table in DEVICE memory lists the
+ * tensors in pieces: _table_chunks() counts its 16-byte entries (negative: an error code), _table_fill() writes them to HOST memory,
+ * the caller copies them to the device once and keeps them while the tensors live.  n elements of dtype VINCE_F32 / VINCE_BF16, dense,
+ * aligned to the element; `scale` stands before the tensor's gradient in the norm (1, or what the optimiser multiplies it by).
+ *   _norm:  norm = sqrt(sum over the tensors of scale^2 sum g^2), sums in fp64;  clip[0] = norm,
+ *           clip[1] = min(1, max_norm / (norm + 1e-6)) (1 for max_norm = infinity; a NaN norm gives NaN, an infinite one 0)
+ *   _scale: every gradient of the table *= clip[1], in place (nothing is written where clip[1] == 1)
+ *   _clip:  _norm, then _scale
+ * scratch: vince_grad_norm_scratch_bytes(), not read before it is written, one for each call in flight.  Fixed order of summation.
+ * vince_sgd_flat_clip: vince_sgd_flat with grad_scale * clip[1] in the place of grad_scale.  (ABI 13) */
+typedef struct vince_grad_tensor {
+    void* data; /* device */
+    int64_t n;
+    float scale;
+    int32_t dtype;
+} vince_grad_tensor;
+int64_t vince_grad_table_chunks(const vince_grad_tensor* tensors /* host */, int32_t count);
+int vince_grad_table_fill(const vince_grad_tensor* tensors /* host */, int32_t count, void* table /* host */, int64_t chunks);
+size_t vince_grad_norm_scratch_bytes(int64_t chunks);
+int vince_grad_norm(const void* table, int64_t chunks, float max_norm, float* clip, void* scratch, size_t scratch_bytes, void* stream);
+int vince_grad_scale(const void* table, int64_t chunks, const float* clip, void* stream);
+int vince_grad_clip(const void* table, int64_t chunks, float max_norm, float* clip, void* scratch, size_t scratch_bytes, void* stream);
+int vince_sgd_flat_clip(float* param, const float* grad, float* buf, int64_t n, float lr, float momentum, float weight_decay,
+                        float grad_scale, const float* clip, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
  * Trunk engine: the ResNet-18/50 trunk (conv1..layer4, backbone_models.py:39-54 with final_layer=-2) + average

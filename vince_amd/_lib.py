@@ -54,6 +54,10 @@ class TrunkCfg(ctypes.Structure):
     _fields_ = [("arch", c_int32), ("N", c_int32), ("H", c_int32), ("W", c_int32), ("dtype", c_int32)]
 
 
+class GradTensor(ctypes.Structure):
+    _fields_ = [("data", c_void_p), ("n", c_int64), ("scale", c_float), ("dtype", c_int32)]
+
+
 P = ctypes.POINTER
 # name -> (restype, argtypes); every symbol declared in include/vince_hip.h
 PROTOTYPES = {
@@ -146,6 +150,18 @@ PROTOTYPES = {
     "vince_queue_enqueue": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, P(c_int64), P(c_int32), c_void_p]),
     "vince_ema_flat": (c_int, [c_void_p, c_void_p, c_int64, c_float, c_void_p]),
     "vince_sgd_flat": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_float, c_float, c_float, c_float, c_void_p]),
+    "vince_layer_norm_fwd": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_float, c_int32,
+                                     c_void_p]),
+    "vince_layer_norm_bwd_scratch_bytes": (c_size_t, [c_int, c_int64, c_int32]),
+    "vince_layer_norm_bwd": (c_int, [c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32,
+                                     c_int64, c_int32, c_void_p, c_size_t, c_void_p]),
+    "vince_grad_table_chunks": (c_int64, [P(GradTensor), c_int32]),
+    "vince_grad_table_fill": (c_int, [P(GradTensor), c_int32, c_void_p, c_int64]),
+    "vince_grad_norm_scratch_bytes": (c_size_t, [c_int64]),
+    "vince_grad_norm": (c_int, [c_void_p, c_int64, c_float, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "vince_grad_scale": (c_int, [c_void_p, c_int64, c_void_p, c_void_p]),
+    "vince_grad_clip": (c_int, [c_void_p, c_int64, c_float, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "vince_sgd_flat_clip": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_float, c_float, c_float, c_float, c_void_p, c_void_p]),
     "vince_trunk_create": (c_int, [P(TrunkCfg), P(c_void_p)]),
     "vince_trunk_destroy": (None, [c_void_p]),
     "vince_trunk_num_params": (c_int32, [c_void_p]),
@@ -180,7 +196,7 @@ _LIB = None
 
 
 # include/vince_hip.h VINCE_ABI_VERSION (tests/test_abi_cpu.py holds the two together)
-ABI_VERSION = 12
+ABI_VERSION = 13
 
 
 def lib():

@@ -1,6 +1,6 @@
 """Flags of the path (reference arg_parser.py:38-241).  Same names and defaults for everything the encoder +
 contrastive path reads; dataset / transform / end-task flags are accepted and ignored so the reference's launch
-scripts (vince/*.sh) parse unchanged.  New: --compute-dtype {bf16,fp32}."""
+scripts (vince/*.sh) parse unchanged.  New: --compute-dtype {bf16,fp32}, --head-norm {none,layer}, --max-grad-norm."""
 import argparse
 import os
 
@@ -55,6 +55,9 @@ def build_parser():
     p.add_argument("--use-apex", action="store_true", help="accepted for script compatibility; use --compute-dtype bf16")
     p.add_argument("--compute-dtype", default="bf16", choices=["bf16", "fp32", "x3", "x3f"],
                    help="trunk arithmetic (head, similarity and loss are always fp32)")
+    p.add_argument("--head-norm", default="none", choices=["none", "layer"],
+                   help="layer: a layer norm between each projection head's first Linear and its ReLU")
+    p.add_argument("--max-grad-norm", default=None, type=float, help="clip the global gradient norm to this (above 0); default: no clipping")
     p.add_argument("--epochs", default=200, type=int)
     p.add_argument("--lr-decay-type", default="cos", choices=["cos", "step"])
     p.add_argument("--lr-step-schedule", default=[120, 160], nargs="*", type=int)

@@ -20,7 +20,7 @@ def make_args(**kw):
         debug=True, title="vince", description="run", num_frames=1, backbone="ResNet18", use_attention=False,
         jigsaw=False, inter_batch_comparison=False, self_batch_comparison=False, batch_size=32, vince_queue_size=512,
         vince_embedding_size=64, vince_momentum=0.999, vince_temperature=0.07, vince_self_temperature=0.03,
-        use_imagenet=False, use_imagenet_weights=False, compute_dtype="fp32", base_lr=0.03, epochs=200,
+        use_imagenet=False, use_imagenet_weights=False, compute_dtype="fp32", head_norm="none", max_grad_norm=None, base_lr=0.03, epochs=200,
         lr_decay_type="cos", lr_step_schedule=[120, 160], use_warmup=True, pytorch_gpu_ids=[0],
         feature_extractor_gpu_ids=[0], input_size=(64, 64), iterations_per_epoch=10, log_frequency=1, save_frequency=10 ** 9,
         long_save_frequency=25, save=False, restore=False, checkpoint_dir=None, long_save_checkpoint_dir=None,

@@ -280,6 +280,17 @@ class VinceModel(BaseModel):
         if args.jigsaw:                                 # nine tile features -> one embedding (vince_model.py:44-49)
             self.jigsaw_linear = nn.Linear(width, width)
             self.jigsaw_embedding = two_layer_head(9 * width, args.vince_embedding_size)
+        # args.head_norm "layer" (--head-norm; not the reference's): a layer norm between each projection head's first Linear and its
+        # ReLU -- per sample, so that nothing of the batch reaches an embedding through the head.  Attributes of their own: the
+        # Linears keep the reference's state-dict keys
+        name = str(getattr(args, "head_norm", None) or "none").lower()
+        if name not in ("none", "layer"):
+            raise ValueError("head_norm must be none or layer, got %r" % name)
+        self.head_norm = name == "layer"
+        if self.head_norm:
+            self.embedding_norm = nn.LayerNorm(width)
+            if args.jigsaw:
+                self.jigsaw_embedding_norm = nn.LayerNorm(width)
         if getattr(args, "use_imagenet", False):        # vince_model.py:79-90: plain torch side heads on detached features
             self.imagenet_decoders = nn.ModuleList([nn.Linear(width, 1000), two_layer_head(width, 1000)])
             self.num_imagenet_decoders = 2
@@ -314,9 +325,13 @@ class VinceModel(BaseModel):
         res = self.feature_extractor.model
         entries = [(p, p.dim() == 4) for p in res.trunk_params]
         heads = [self.embedding[0].weight, self.embedding[0].bias, self.embedding[2].weight, self.embedding[2].bias]
+        if self.head_norm:
+            heads += [self.embedding_norm.weight, self.embedding_norm.bias]
         if self.args.jigsaw:
             heads += [self.jigsaw_linear.weight, self.jigsaw_linear.bias, self.jigsaw_embedding[0].weight,
                       self.jigsaw_embedding[0].bias, self.jigsaw_embedding[2].weight, self.jigsaw_embedding[2].bias]
+            if self.head_norm:
+                heads += [self.jigsaw_embedding_norm.weight, self.jigsaw_embedding_norm.bias]
         entries += [(p, False) for p in heads]
         tail = [(res.fc.weight, False), (res.fc.bias, False)]
         return entries, tail
@@ -354,7 +369,8 @@ class VinceModel(BaseModel):
         self._head_params = [p for p, _ in entries[ntrunk:]]
         # contiguous flat ranges by role: SGD skips a head whose parameters received no gradient this step, exactly as
         # torch.optim.SGD skips parameters whose .grad is None (the standard head idles when the query side is jigsawed)
-        emb_end = offs[ntrunk + 4] if len(entries) > ntrunk + 4 else n_train
+        n_emb = 6 if self.head_norm else 4
+        emb_end = offs[ntrunk + n_emb] if len(entries) > ntrunk + n_emb else n_train
         self._segments = {"trunk": (0, offs[ntrunk]), "embedding": (offs[ntrunk], emb_end), "jigsaw": (emb_end, n_train)}
         self._touched = {"trunk": False, "embedding": False, "jigsaw": False}
         self._bucket_events = None
@@ -421,6 +437,10 @@ class VinceModel(BaseModel):
         params = list(self.feature_extractor.parameters()) + list(self.embedding.parameters())
         if self.args.jigsaw:
             params += list(self.jigsaw_linear.parameters()) + list(self.jigsaw_embedding.parameters())
+        if self.head_norm:
+            params += list(self.embedding_norm.parameters())
+            if self.args.jigsaw:
+                params += list(self.jigsaw_embedding_norm.parameters())
         return params
 
     # ------------------------------------------------------------------------------------------ engine plumbing
@@ -590,16 +610,24 @@ class VinceModel(BaseModel):
                 if hx3 and _head_x3_shape(layer.weight):
                     return ops.linear_fwd(x, self._head_c.copies(id(layer.weight), bool(save))[0], layer.bias.data, relu=relu, x3="b")
                 return ops.linear_fwd(x, layer.weight.data, layer.bias.data, relu=relu)
+
+            def hidden(x, layer, norm):      # Linear [+ layer norm] + ReLU
+                if norm is None:
+                    return lin(x, layer, relu=True)
+                h = lin(x, layer)
+                out, mean, rstd = ops.layer_norm_fwd(h, norm.weight.data, norm.bias.data, norm.eps, relu=True)
+                saved.update(normed=(h, mean, rstd))
+                return out
             if jigsaw:   # vince_model.py:161-171
                 f = lin(pooled, self.jigsaw_linear)
                 c = f.shape[1]
                 idx = orders.to(f.device).unsqueeze(-1).expand(n, 9, c)
                 g = torch.gather(f.view(n, 9, c), 1, idx).reshape(n, 9 * c).contiguous()
-                hid = lin(g, self.jigsaw_embedding[0], relu=True)
+                hid = hidden(g, self.jigsaw_embedding[0], self.jigsaw_embedding_norm if self.head_norm else None)
                 pre = lin(hid, self.jigsaw_embedding[2])
                 saved.update(g=g, hid=hid, orders=orders.to(f.device))
             else:        # vince_model.py:175-177
-                hid = lin(pooled, self.embedding[0], relu=True)
+                hid = hidden(pooled, self.embedding[0], self.embedding_norm if self.head_norm else None)
                 pre = lin(hid, self.embedding[2])
                 saved.update(hid=hid)
             emb, norms = ops.l2norm_fwd(pre)   # F.normalize(dim=1), vince_model.py:180
@@ -630,10 +658,17 @@ class VinceModel(BaseModel):
                 if hx3 and _head_x3_shape(w):
                     return ops.linear_bwd(x, self._head_c.copies(id(w), True)[1], dy, hg[id(w)], hg[id(layer.bias)], x3=True)
                 return ops.linear_bwd(x, ht[id(w)], dy, hg[id(w)], hg[id(layer.bias)])
+
+            def hidden_bwd(dh, norm):        # through the ReLU [and the layer norm] behind a head's first Linear
+                if norm is None:
+                    return ops.relu_bwd(dh, s["hid"])
+                h, mean, rstd = s["normed"]
+                return ops.layer_norm_bwd(h, norm.weight.data, mean, rstd, dh, act=s["hid"], dweight=hg[id(norm.weight)],
+                                          dbias=hg[id(norm.bias)])[0]
             if s["jigsaw"]:
                 l0, l2, lj = self.jigsaw_embedding[0], self.jigsaw_embedding[2], self.jigsaw_linear
                 dh = lbwd(s["hid"], l2, dpre)
-                dh = ops.relu_bwd(dh, s["hid"])
+                dh = hidden_bwd(dh, self.jigsaw_embedding_norm if self.head_norm else None)
                 dg = lbwd(s["g"], l0, dh)
                 n, c = dg.shape[0], dg.shape[1] // 9
                 df = torch.zeros(n, 9, c, device=dg.device)
@@ -643,7 +678,7 @@ class VinceModel(BaseModel):
             else:
                 l0, l2 = self.embedding[0], self.embedding[2]
                 dh = lbwd(s["hid"], l2, dpre)
-                dh = ops.relu_bwd(dh, s["hid"])
+                dh = hidden_bwd(dh, self.embedding_norm if self.head_norm else None)
                 dp = lbwd(s["pooled"], l0, dh)
             dpool_total = dp if dpool_total is None else dpool_total + dp
         if dpool_total is None:

@@ -8,7 +8,7 @@ import ctypes
 import torch
 
 from . import _lib
-from ._lib import BnReduce, BnTrain, ConvDesc, ConvEpi, InfoNCEDesc, VINCE_BF16, VINCE_F32, VINCE_F32X1B, VINCE_F32X3B, VINCE_F32X3H, check, lib
+from ._lib import BnReduce, BnTrain, ConvDesc, ConvEpi, GradTensor, InfoNCEDesc, VINCE_BF16, VINCE_F32, VINCE_F32X1B, VINCE_F32X3B, VINCE_F32X3H, check, lib
 
 EPI_ACCUMULATE, EPI_RELU, EPI_IN_HALF_PAIRS = _lib.EPI_ACCUMULATE, _lib.EPI_RELU, _lib.EPI_IN_HALF_PAIRS
 STATS_REPLICAS = 16   # VINCE_STATS_REPLICAS in include/vince_hip.h
@@ -42,6 +42,30 @@ def require_gpu(*tensors):
             raise RuntimeError("vince_amd: tensor on %s -- the HIP path needs GPU tensors (no CPU fallback)" % t.device)
         if not t.is_contiguous():
             raise RuntimeError("vince_amd: tensor must be contiguous")
+
+
+def _one_gpu(*tensors):
+    """The device that every given tensor (None: not given) is on; contiguous GPU tensors only."""
+    dev = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda or not t.is_contiguous():
+            require_gpu(t)
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise RuntimeError("vince_amd: tensors on %s and %s -- one call works on one GPU" % (dev, t.device))
+    return dev
+
+
+def _launch(dev, fn, *args):
+    """fn(*args, stream) on the current stream of `dev`, whichever device is current."""
+    if dev.index == torch.cuda.current_device():
+        check(fn(*args, torch.cuda.current_stream().cuda_stream))
+    else:
+        with torch.cuda.device(dev):
+            check(fn(*args, torch.cuda.current_stream().cuda_stream))
 
 
 # ------------------------------------------------------------------------------------------------ conv descriptors
@@ -357,6 +381,67 @@ def l2norm_bwd(x, norms, dout, eps=1e-12):
 
 
 # ------------------------------------------------------------------------------------------------ batch norm / pooling
+def _layer_norm_vectors(what, cols, **vectors):
+    for name, v in vectors.items():
+        if v is not None and (v.dtype != torch.float32 or v.shape != (cols,)):
+            raise ValueError("%s: %s has to be float32 [%d], got %s %s" % (what, name, cols, v.dtype, tuple(v.shape)))
+
+
+def layer_norm_fwd(x, weight=None, bias=None, eps=1e-5, relu=False):
+    """Layer norm over the last axis of x [..., D] (float32 or bfloat16): (x - mean) * rstd * weight + bias, rstd = 1 / sqrt(var + eps)
+    with the biased variance; relu: max(., 0) in the same pass.  weight, bias: float32 [D] or None (no bias without a weight).
+    Returns (out like x, mean float32 [...], rstd float32 [...]); layer_norm_bwd takes the last two."""
+    dev = _one_gpu(x, weight, bias)
+    code = dtype_code(x)
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise ValueError("layer_norm_fwd: x has no last axis to normalise, got shape %s" % (tuple(x.shape),))
+    if weight is None and bias is not None:
+        raise ValueError("layer_norm_fwd: a bias without a weight")
+    if not eps >= 0:
+        raise ValueError("layer_norm_fwd: eps=%r" % (eps,))
+    cols = x.shape[-1]
+    _layer_norm_vectors("layer_norm_fwd", cols, weight=weight, bias=bias)
+    out = torch.empty_like(x)
+    mean = torch.empty(x.shape[:-1], device=dev, dtype=torch.float32)
+    rstd = torch.empty_like(mean)
+    _launch(dev, lib().vince_layer_norm_fwd, code, x.data_ptr(), None if weight is None else weight.data_ptr(),
+            None if bias is None else bias.data_ptr(), out.data_ptr(), mean.data_ptr(), rstd.data_ptr(), mean.numel(), cols, eps, int(relu))
+    return out, mean, rstd
+
+
+def layer_norm_bwd(x, weight, mean, rstd, dout, act=None, dweight=None, dbias=None):
+    """Gradients of layer_norm_fwd from its input x, weight, mean and rstd and the output's gradient `dout` (type and shape of x).
+    act: the output of a forward with relu=True -- dout counts as zero where act <= 0 (as ops.relu_bwd has it).
+    dweight, dbias: float32 [D] buffers the parameters' gradients are ADDED to (as ops.linear_bwd does); without them they are returned
+    in new tensors.  Without a weight there are neither.  Returns (dx, dweight, dbias).  Same bits on every call: no atomics."""
+    dev = _one_gpu(x, weight, mean, rstd, dout, act, dweight, dbias)
+    code = dtype_code(x)
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise ValueError("layer_norm_bwd: x has no last axis, got shape %s" % (tuple(x.shape),))
+    for name, t in (("dout", dout), ("act", act)):
+        if t is not None and (t.dtype != x.dtype or t.shape != x.shape):
+            raise ValueError("layer_norm_bwd: %s is %s %s, x is %s %s" % (name, t.dtype, tuple(t.shape), x.dtype, tuple(x.shape)))
+    cols = x.shape[-1]
+    for name, t in (("mean", mean), ("rstd", rstd)):
+        if t.dtype != torch.float32 or t.numel() * cols != x.numel():
+            raise ValueError("layer_norm_bwd: %s has to hold one float32 per row of x, got %s %s" % (name, t.dtype, tuple(t.shape)))
+    if (dweight is None) != (dbias is None) or (weight is None and dweight is not None):
+        raise ValueError("layer_norm_bwd: dweight and dbias come together, and with a weight")
+    _layer_norm_vectors("layer_norm_bwd", cols, weight=weight, dweight=dweight, dbias=dbias)
+    accumulate = dweight is not None
+    if weight is not None and not accumulate:
+        dweight, dbias = torch.empty_like(weight), torch.empty_like(weight)
+    rows = mean.numel()
+    dx = torch.empty_like(x)
+    nbytes = 0 if weight is None else lib().vince_layer_norm_bwd_scratch_bytes(code, rows, cols)
+    scratch = torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
+    _launch(dev, lib().vince_layer_norm_bwd, code, x.data_ptr(), None if weight is None else weight.data_ptr(), mean.data_ptr(),
+            rstd.data_ptr(), dout.data_ptr(), None if act is None else act.data_ptr(), dx.data_ptr(),
+            None if dweight is None else dweight.data_ptr(), None if dbias is None else dbias.data_ptr(), int(accumulate), rows, cols,
+            None if scratch is None else scratch.data_ptr(), nbytes)
+    return dx, dweight, dbias
+
+
 def bn_finalize(stats, count, gamma, beta, running_mean, running_var, nbt, train, momentum=0.1, eps=1e-5):
     C = gamma.numel()
     consts = torch.empty(4, C, device=gamma.device, dtype=torch.float32)
@@ -667,10 +752,120 @@ def ema_flat(key, query, momentum):
     check(lib().vince_ema_flat(_ptr(key), _ptr(query), key.numel(), momentum, stream_ptr()))
 
 
-def sgd_flat(param, grad, buf, lr, momentum=0.9, weight_decay=1e-4, grad_scale=1.0):
+def sgd_flat(param, grad, buf, lr, momentum=0.9, weight_decay=1e-4, grad_scale=1.0, clip=None):
+    """clip: what grad_norm returned -- the gradient is scaled by clip[1] too, without being rewritten."""
+    if clip is not None:
+        dev = _one_gpu(param, grad, buf, clip)
+        if not (param.dtype == grad.dtype == buf.dtype == clip.dtype == torch.float32) or clip.numel() != 2:
+            raise TypeError("vince_amd: sgd_flat takes float32 tensors, and a clip of two values (grad_norm)")
+        if not param.numel() == grad.numel() == buf.numel():
+            raise ValueError("vince_amd: sgd_flat: %d parameters, %d gradients, %d momentum values"
+                             % (param.numel(), grad.numel(), buf.numel()))
+        _launch(dev, lib().vince_sgd_flat_clip, param.data_ptr(), grad.data_ptr(), buf.data_ptr(), param.numel(), lr, momentum, weight_decay,
+                grad_scale, clip.data_ptr())
+        return
     require_gpu(param, grad, buf)
     check(lib().vince_sgd_flat(_ptr(param), _ptr(grad), _ptr(buf), param.numel(), lr, momentum, weight_decay, grad_scale,
                                stream_ptr()))
+
+
+# ------------------------------------------------------------------------------------------------ gradient norm and clipping
+def _dense(t):
+    """Whether t's elements fill one block of memory, in any order of the axes, each at a place of its own."""
+    if t.is_contiguous():
+        return True
+    want = 1
+    for stride, size in sorted((st, n) for n, st in zip(t.shape, t.stride()) if n != 1):
+        if stride != want:
+            return False
+        want *= size
+    return True
+
+
+class GradTable:
+    """A list of gradient tensors laid out once for grad_norm / grad_clip / grad_scale: keep it as long as the gradients keep their
+    memory (VinceModel's do: views of its flat buffer), make a new one when one of them gets another.
+
+    tensors: float32 or bfloat16 GPU tensors on one device, dense in any order of their axes (channels_last gradients are), not
+    overlapping, empty ones allowed.  scales: what stands before each tensor in the norm (default 1), e.g. the grad_scale of the step.
+    The table holds its tensors; a captured graph that uses it needs it alive for every replay, and it has to be made before the capture.
+    One table may be used from several streams at once, as far as its gradients may."""
+
+    def __init__(self, tensors, scales=None):
+        self.tensors = list(tensors)
+        scales = [1.0] * len(self.tensors) if scales is None else [float(v) for v in scales]
+        if not self.tensors or len(scales) != len(self.tensors):
+            raise ValueError("GradTable: %d tensors, %d scales" % (len(self.tensors), len(scales)))
+        self.device = self.tensors[0].device
+        entries, spans = (GradTensor * len(self.tensors))(), []
+        for i, t in enumerate(self.tensors):
+            if not t.is_cuda:
+                raise RuntimeError("vince_amd: tensor on %s -- the HIP path needs GPU tensors (no CPU fallback)" % t.device)
+            if t.device != self.device:
+                raise RuntimeError("vince_amd: tensors on %s and %s -- one table is for one GPU" % (self.device, t.device))
+            if not _dense(t):
+                raise ValueError("GradTable: tensor %d (shape %s, strides %s) is not dense" % (i, tuple(t.shape), t.stride()))
+            entries[i] = GradTensor(data=t.data_ptr(), n=t.numel(), scale=scales[i], dtype=dtype_code(t))
+            if t.numel():
+                spans.append((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()))
+        spans.sort()
+        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+            raise ValueError("GradTable: two of the tensors share memory")
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("vince_amd: a GradTable is copied to the GPU when it is made: make it before the capture")
+        self.chunks = lib().vince_grad_table_chunks(entries, len(self.tensors))
+        check(min(self.chunks, 0))
+        host = torch.empty(self.chunks, 2, dtype=torch.int64)
+        check(lib().vince_grad_table_fill(entries, len(self.tensors), host.data_ptr(), self.chunks))
+        self._table = host.to(self.device)            # (synchronous: any stream may read it from here on)
+        self._scratch_bytes = lib().vince_grad_norm_scratch_bytes(self.chunks)
+        with torch.cuda.device(self.device):
+            self._stream = torch.cuda.current_stream().cuda_stream
+
+    def _run(self, fn, *args):
+        def go():
+            stream = torch.cuda.current_stream()
+            if stream.cuda_stream != self._stream:     # (its memory outlives what this stream still has to read)
+                self._table.record_stream(stream)
+            check(fn(self._table.data_ptr(), self.chunks, *args, stream.cuda_stream))
+        if self.device.index == torch.cuda.current_device():
+            go()
+        else:
+            with torch.cuda.device(self.device):
+                go()
+
+    def _norm(self, fn, max_norm):
+        max_norm = float("inf") if max_norm is None else float(max_norm)
+        if not max_norm >= 0:
+            raise ValueError("vince_amd: max_norm=%r" % (max_norm,))
+        clip = torch.empty(2, device=self.device, dtype=torch.float32)
+        scratch = torch.empty(self._scratch_bytes, device=self.device, dtype=torch.uint8)    # (a call's own: two may be in flight)
+        self._run(fn, max_norm, clip.data_ptr(), scratch.data_ptr(), self._scratch_bytes)
+        return clip
+
+
+def _grad_table(grads):
+    return grads if isinstance(grads, GradTable) else GradTable(grads)
+
+
+def grad_norm(grads, max_norm=None):
+    """The 2-norm over all gradients (a GradTable, or tensors to make one of): float32 [norm, coefficient] on the GPU, coefficient =
+    min(1, max_norm / (norm + 1e-6)), 1 without a max_norm.  Sums are fp64 in a fixed order.  A gradient that is not finite shows as
+    a norm of inf or NaN and a coefficient of 0 or NaN; nothing raises, nothing synchronises."""
+    return _grad_table(grads)._norm(lib().vince_grad_norm, max_norm)
+
+
+def grad_clip(grads, max_norm):
+    """grad_norm, then every gradient times the coefficient, in place.  Returns the same [norm, coefficient] (the norm before)."""
+    return _grad_table(grads)._norm(lib().vince_grad_clip, max_norm)
+
+
+def grad_scale(grads, clip):
+    """Every gradient times clip[1], in place: for gradients that another call's norm includes."""
+    table = _grad_table(grads)
+    if _one_gpu(clip) != table.device or clip.dtype != torch.float32 or clip.numel() != 2:
+        raise ValueError("grad_scale: clip is what grad_norm returns (float32 [2]) on %s" % (table.device,))
+    table._run(lib().vince_grad_scale, clip.data_ptr())
 
 
 # ------------------------------------------------------------------------------------------------ GPU input stage (csrc/augment.hip)

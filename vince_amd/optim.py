@@ -9,6 +9,11 @@ that was never run).  Once a range has been used it is stepped on every later st
 torch==1.4.0 (requirements.txt:17), whose ``optimizer.zero_grad()`` zeroes gradients in place and never resets them to
 None, so under ``--jigsaw`` alternation the idle head keeps receiving weight decay and momentum with a zero gradient.
 Parameters outside the flat buffer (the optional ImageNet side decoders) go through a plain torch SGD.
+
+``max_grad_norm`` (--max-grad-norm): the step is taken with every gradient scaled by min(1, max_grad_norm / (norm + 1e-6)), norm =
+the 2-norm over all gradients the step applies (``grad_scale`` included), as torch.nn.utils.clip_grad_norm_ before a plain SGD would
+have it.  The norm is one pass over the flat buffer on the device; the SGD kernel reads the coefficient there, so the gradients in the
+buffer are not rewritten (those of the side decoders are).  ``last_clip`` holds [norm, coefficient] of the last step, on the device.
 """
 import torch
 
@@ -16,8 +21,12 @@ from . import ops
 
 
 class FlatSGD:
-    def __init__(self, model, lr, momentum=0.9, weight_decay=1e-4):
+    def __init__(self, model, lr, momentum=0.9, weight_decay=1e-4, max_grad_norm=None):
         self.model = model
+        if max_grad_norm is not None and not max_grad_norm > 0:
+            raise ValueError("FlatSGD: max_grad_norm has to be above 0, got %r" % (max_grad_norm,))
+        self.max_grad_norm, self.last_clip = max_grad_norm, None
+        self._clip_table = self._extra_table = None
         self.momentum, self.weight_decay = momentum, weight_decay
         self.param_groups = [{"params": list(model.parameters()), "lr": lr, "initial_lr": lr, "momentum": momentum,
                               "weight_decay": weight_decay}]
@@ -31,11 +40,40 @@ class FlatSGD:
     def zero_grad(self, set_to_none=True):
         self.model.zero_grad()
 
+    def _same_memory(self, table, grads, scales):
+        """Whether `table` lists exactly these gradients: it holds its tensors, so their memory cannot have been handed out again."""
+        return table is not None and self._clip_scales == scales and len(table.tensors) == len(grads) and all(
+            a.data_ptr() == b.data_ptr() and a.numel() == b.numel() for a, b in zip(table.tensors, grads))
+
+    def _clip(self, grad):
+        """[norm, coefficient] over every gradient this step applies; scales the gradients outside the flat buffer in place.  Needs them
+        all: waits (on the device) for what a deferred stem join or a late gradient bucket still has in flight."""
+        late = getattr(self.model, "_late", None)
+        if late:
+            late[1]()
+            self.model._late = None
+        self.model.finish_stem_grad()
+        grads = [grad[a:b] for role, (a, b) in self.model._segments.items() if b > a and role in self._ever_touched]
+        extra = [] if self._extra is None else [p.grad for g in self._extra.param_groups for p in g["params"] if p.grad is not None]
+        if not grads and not extra:
+            return None
+        # (the flat buffer holds sums over the ranks and grad_scale makes means of them; the side decoders' gradients are means already)
+        scales = [float(self.grad_scale)] * len(grads) + [1.0] * len(extra)
+        if not self._same_memory(self._clip_table, grads + extra, scales):
+            self._clip_scales = scales
+            self._clip_table = ops.GradTable(grads + extra, scales)
+            self._extra_table = ops.GradTable(extra) if extra else None
+        clip = ops.grad_norm(self._clip_table, self.max_grad_norm)
+        if extra:
+            ops.grad_scale(self._extra_table, clip)
+        return clip
+
     def step(self, defer_stem=False):
         """defer_stem=True (VinceSolver's loop; only meaningful when the model runs with defer_stem_join): every parameter but
         conv1.weight is stepped now -- beside the stem's weight gradient, still running on the engine's side stream -- and
         conv1.weight's own step is left as model._deferred_step, which VinceQueueModel.param_update / the next forward / zero_grad
-        finish behind the stem event.  The default completes everything before returning."""
+        finish behind the stem event.  The default completes everything before returning, and so does a step with max_grad_norm, whose
+        coefficient depends on every gradient."""
         lr = float(self.param_groups[0]["lr"])
         flat, grad, n_train, _ = self.model.flat_parameters()
         if self.momentum_buffer.device != flat.device:
@@ -44,9 +82,11 @@ class FlatSGD:
             grad.zero_()
             self.model._grad_zero_pending = False
         deferred_trunk = None
-        for role, (a, b) in self.model._segments.items():
+        for role in self.model._segments:
             if self.model._touched.get(role, False):
                 self._ever_touched.add(role)
+        clip = self.last_clip = None if self.max_grad_norm is None else self._clip(grad)
+        for role, (a, b) in self.model._segments.items():
             # an idle range's flat gradient is all zeros here (the whole buffer is cleared before backward): the kernel then
             # applies exactly weight decay + momentum, which is what torch 1.4 does with an in-place-zeroed .grad
             if b > a and role in self._ever_touched:
@@ -78,7 +118,7 @@ class FlatSGD:
                         finish()
                     continue
                 ops.sgd_flat(flat[a:b], grad[a:b], self.momentum_buffer[a:b], lr, self.momentum, self.weight_decay,
-                             self.grad_scale)
+                             self.grad_scale, clip=clip)
         if deferred_trunk is not None and self.model._deferred_split == self.model._offs[1]:
             # every parameter but conv1.weight has its new value: rebuild their compute copies now, beside the stem's weight gradient
             # (the head ranges were stepped by the launches above; the trunk's table entry 0 follows in finish())
@@ -101,5 +141,6 @@ class FlatSGD:
 
     def __repr__(self):
         g = self.param_groups[0]
-        return "FlatSGD(lr=%g, momentum=%g, weight_decay=%g, flat_params=%d)" % (
-            g["lr"], self.momentum, self.weight_decay, self.momentum_buffer.numel())
+        limit = "" if self.max_grad_norm is None else ", max_grad_norm=%g" % self.max_grad_norm
+        return "FlatSGD(lr=%g, momentum=%g, weight_decay=%g, flat_params=%d%s)" % (
+            g["lr"], self.momentum, self.weight_decay, self.momentum_buffer.numel(), limit)

@@ -104,7 +104,8 @@ class VinceSolver(BaseSolver):
 
     def setup_optimizer(self):
         # vince_solver.py:252-265: SGD(lr=base_lr, weight_decay=1e-4, momentum=0.9) on model.parameters()
-        self.optimizer = FlatSGD(self.model, lr=self.args.base_lr, momentum=0.9, weight_decay=0.0001)
+        self.optimizer = FlatSGD(self.model, lr=self.args.base_lr, momentum=0.9, weight_decay=0.0001,
+                                 max_grad_norm=getattr(self.args, "max_grad_norm", None))
         w, _ = dp.world()
         if w > 1 or (os.environ.get("VINCE_FORCE_DP") and torch.distributed.is_initialized()):
             # (VINCE_FORCE_DP exercises the bucketed all-reduce machinery with a single-rank process group)
@@ -481,6 +482,8 @@ class VinceSolver(BaseSolver):
                 record = {"times/%s/%s" % (tag, k): m.val for k, m in self.time_meters.items()}
                 record.update({"losses/%s/%s" % (tag, k): self.loss_meters[k].val for k in updated_loss_meters})
                 record.update({"metrics/%s/%s" % (tag, k): self.metric_meters[k].val for k in metrics})
+                if getattr(self.optimizer, "last_clip", None) is not None:      # (--max-grad-norm: the norm before clipping)
+                    record["metrics/%s/grad_norm" % tag] = float(self.optimizer.last_clip[0])
                 self.train_logger.dict_log(record, self.iteration)
 
         if step_no % self.args.save_frequency == 0:
