@@ -16,6 +16,11 @@ struct GradChunk {
 };
 static_assert(sizeof(GradChunk) == 16, "the table's layout is the header's");
 
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(bf16_t v) { return bf16_to_f32(v); }
+__device__ __forceinline__ void put(float* p, float v) { *p = v; }
+__device__ __forceinline__ void put(bf16_t* p, float v) { *p = f32_to_bf16(v); }
+
 __device__ __forceinline__ double block_sum(double v) {
     __shared__ double red[4];
 #pragma unroll
@@ -26,50 +31,128 @@ __device__ __forceinline__ double block_sum(double v) {
     return (red[0] + red[1]) + (red[2] + red[3]);
 }
 
+// 16 bytes from an address aligned to the element only (the hardware takes any; the type tells the compiler so).  The table's addresses
+// are device memory: said to the compiler too, which would otherwise make flat accesses of them.
+typedef __attribute__((ext_vector_type(4), aligned(2))) uint32_t u32x4_any_t;
+typedef __attribute__((address_space(1))) u32x4_any_t global_u32x4_any_t;
+__device__ __forceinline__ uint4 load16(const void* p) {
+    const u32x4_any_t v = *(const global_u32x4_any_t*)p;
+    return make_uint4(v[0], v[1], v[2], v[3]);
+}
+__device__ __forceinline__ void store16(void* p, const uint4& v) {
+    const u32x4_any_t w = {v.x, v.y, v.z, v.w};
+    *(global_u32x4_any_t*)p = w;
+}
+
+template <typename T> __device__ __forceinline__ double squares_of(const T* __restrict__ g, int n) {
+    constexpr int V = Elem<T>::CH, STEP = 256 * V, DEEP = 4;
+    double s0 = 0.0, s1 = 0.0;
+    int i = threadIdx.x * V;
+    for (; i + (DEEP - 1) * STEP + V <= n; i += DEEP * STEP) {       // DEEP loads are in flight before the first is used
+        uint4 q[DEEP];
+#pragma unroll
+        for (int d = 0; d < DEEP; ++d) q[d] = load16(g + i + d * STEP);
+#pragma unroll
+        for (int d = 0; d < DEEP; ++d) {
+            float f[V];
+            Chunk<T>::unpack(q[d], f);
+#pragma unroll
+            for (int e = 0; e < V; e += 2) {
+                s0 = fma((double)f[e], (double)f[e], s0);
+                s1 = fma((double)f[e + 1], (double)f[e + 1], s1);
+            }
+        }
+    }
+    for (; i < n; i += STEP) {
+        if (i + V <= n) {
+            float f[V];
+            Chunk<T>::unpack(load16(g + i), f);
+#pragma unroll
+            for (int e = 0; e < V; ++e) s0 = fma((double)f[e], (double)f[e], s0);
+        } else {
+            for (int j = i; j < n; ++j) {
+                const double v = to_float(g[j]);
+                s1 = fma(v, v, s1);
+            }
+        }
+    }
+    return s0 + s1;
+}
+
 __global__ __launch_bounds__(256) void grad_squares_kernel(const GradChunk* __restrict__ table, int64_t chunks, double* __restrict__ partial) {
     double sum = 0.0;
     for (int64_t c = blockIdx.x; c < chunks; c += gridDim.x) {
         const GradChunk k = table[c];
         const int n = (int)(k.n & ~GRAD_BF16);
-        double s = 0.0;
-        if (k.n & GRAD_BF16) {
-            const bf16_t* g = (const bf16_t*)k.data;
-            for (int i = threadIdx.x; i < n; i += 256) { const double v = bf16_to_f32(g[i]); s = fma(v, v, s); }
-        } else {
-            const float* g = (const float*)k.data;
-            for (int i = threadIdx.x; i < n; i += 256) { const double v = g[i]; s = fma(v, v, s); }
-        }
+        const double s = k.n & GRAD_BF16 ? squares_of((const bf16_t*)k.data, n) : squares_of((const float*)k.data, n);
         sum = fma((double)k.scale * (double)k.scale, s, sum);
     }
     sum = block_sum(sum);
     if (threadIdx.x == 0) partial[blockIdx.x] = sum;
 }
 
-// clip[0] = norm, clip[1] = min(1, max_norm / (norm + 1e-6)); an infinite max_norm clips nothing, a NaN norm gives a NaN coefficient
-__global__ __launch_bounds__(256) void grad_clip_kernel(const double* __restrict__ partial, int n, float max_norm, float* __restrict__ clip) {
+// [norm, coefficient] from the workgroups' sums, by every thread of a workgroup of 256: norm = sqrt(sum), coefficient =
+// min(1, max_norm / (norm + 1e-6)); an infinite max_norm clips nothing, a NaN norm gives a NaN coefficient
+__device__ __forceinline__ float2 clip_of(const double* __restrict__ partial, int n, float max_norm) {
     double s = 0.0;
     for (int i = threadIdx.x; i < n; i += 256) s += partial[i];
-    s = block_sum(s);
-    if (threadIdx.x == 0) {
-        const double norm = sqrt(s), c = (double)max_norm / (norm + 1e-6);
-        clip[0] = (float)norm;
-        clip[1] = max_norm == INFINITY || c > 1.0 ? 1.f : (float)c;
+    const double norm = sqrt(block_sum(s)), c = (double)max_norm / (norm + 1e-6);
+    return make_float2((float)norm, max_norm == INFINITY || c > 1.0 ? 1.f : (float)c);
+}
+
+__global__ __launch_bounds__(256) void grad_clip_kernel(const double* __restrict__ partial, int n, float max_norm, float* __restrict__ clip) {
+    const float2 r = clip_of(partial, n, max_norm);
+    if (threadIdx.x == 0) { clip[0] = r.x; clip[1] = r.y; }
+}
+
+template <typename T> __device__ __forceinline__ void scale_piece(T* __restrict__ g, int n, float f) {
+    constexpr int V = Elem<T>::CH, STEP = 256 * V, DEEP = 4;
+    int i = threadIdx.x * V;
+    for (; i + (DEEP - 1) * STEP + V <= n; i += DEEP * STEP) {
+        uint4 q[DEEP];
+#pragma unroll
+        for (int d = 0; d < DEEP; ++d) q[d] = load16(g + i + d * STEP);
+#pragma unroll
+        for (int d = 0; d < DEEP; ++d) {
+            float v[V];
+            Chunk<T>::unpack(q[d], v);
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[e] *= f;
+            store16(g + i + d * STEP, Chunk<T>::pack(v));
+        }
+    }
+    for (; i < n; i += STEP) {
+        if (i + V <= n) {
+            float v[V];
+            Chunk<T>::unpack(load16(g + i), v);
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[e] *= f;
+            store16(g + i, Chunk<T>::pack(v));
+        } else {
+            for (int j = i; j < n; ++j) put(g + j, to_float(g[j]) * f);
+        }
     }
 }
 
-__global__ __launch_bounds__(256) void grad_scale_kernel(const GradChunk* __restrict__ table, int64_t chunks, const float* __restrict__ clip) {
-    const float f = clip[1];
+// FINAL: the coefficient comes from the sums of grad_squares_kernel, added up by every workgroup for itself (8 KB at most, in the
+// caches) -- one launch fewer than a kernel of its own for it; else from clip[1]
+template <bool FINAL>
+__global__ __launch_bounds__(256) void grad_scale_kernel(const GradChunk* __restrict__ table, int64_t chunks, float* __restrict__ clip,
+                                                         const double* __restrict__ partial, int n_partial, float max_norm) {
+    float f;
+    if constexpr (FINAL) {
+        const float2 r = clip_of(partial, n_partial, max_norm);
+        if (blockIdx.x == 0 && threadIdx.x == 0) { clip[0] = r.x; clip[1] = r.y; }
+        f = r.y;
+    } else {
+        f = clip[1];
+    }
     if (f == 1.f) return;                  // every product would be the gradient itself
     for (int64_t c = blockIdx.x; c < chunks; c += gridDim.x) {
         const GradChunk k = table[c];
         const int n = (int)(k.n & ~GRAD_BF16);
-        if (k.n & GRAD_BF16) {
-            bf16_t* g = (bf16_t*)k.data;
-            for (int i = threadIdx.x; i < n; i += 256) g[i] = f32_to_bf16(bf16_to_f32(g[i]) * f);
-        } else {
-            float* g = (float*)k.data;
-            for (int i = threadIdx.x; i < n; i += 256) g[i] *= f;
-        }
+        if (k.n & GRAD_BF16) scale_piece((bf16_t*)k.data, n, f);
+        else scale_piece((float*)k.data, n, f);
     }
 }
 
@@ -137,10 +220,13 @@ extern "C" int vince_grad_table_fill(const vince_grad_tensor* tensors, int32_t c
 
 extern "C" size_t vince_grad_norm_scratch_bytes(int64_t chunks) { return chunks > 0 ? (size_t)grad_blocks(chunks) * sizeof(double) : 0; }
 
+#define GRAD_NORM_CHECK(name)                                                                                                              \
+    VINCE_CHECK_ARG(chunks >= 0 && clip && (chunks == 0 || (table && scratch)), VINCE_E_ARG, name ": bad arguments");                      \
+    VINCE_CHECK_ARG(max_norm >= 0.f, VINCE_E_ARG, name ": max_norm=%g", (double)max_norm);                                                 \
+    VINCE_CHECK_ARG(scratch_bytes >= vince_grad_norm_scratch_bytes(chunks), VINCE_E_ARG, name ": scratch of %zu bytes", scratch_bytes)
+
 extern "C" int vince_grad_norm(const void* table, int64_t chunks, float max_norm, float* clip, void* scratch, size_t scratch_bytes, void* stream) {
-    VINCE_CHECK_ARG(chunks >= 0 && clip && (chunks == 0 || (table && scratch)), VINCE_E_ARG, "vince_grad_norm: bad arguments");
-    VINCE_CHECK_ARG(max_norm >= 0.f, VINCE_E_ARG, "vince_grad_norm: max_norm=%g", (double)max_norm);
-    VINCE_CHECK_ARG(scratch_bytes >= vince_grad_norm_scratch_bytes(chunks), VINCE_E_ARG, "vince_grad_norm: scratch of %zu bytes", scratch_bytes);
+    GRAD_NORM_CHECK("vince_grad_norm");
     const int blocks = grad_blocks(chunks);
     if (blocks > 0)
         hipLaunchKernelGGL(grad_squares_kernel, dim3(blocks), dim3(256), 0, (hipStream_t)stream, (const GradChunk*)table, chunks, (double*)scratch);
@@ -152,14 +238,21 @@ extern "C" int vince_grad_norm(const void* table, int64_t chunks, float max_norm
 extern "C" int vince_grad_scale(const void* table, int64_t chunks, const float* clip, void* stream) {
     VINCE_CHECK_ARG(chunks >= 0 && clip && (chunks == 0 || table), VINCE_E_ARG, "vince_grad_scale: bad arguments");
     if (chunks == 0) return VINCE_OK;
-    hipLaunchKernelGGL(grad_scale_kernel, dim3(grad_blocks(chunks)), dim3(256), 0, (hipStream_t)stream, (const GradChunk*)table, chunks, clip);
+    hipLaunchKernelGGL(grad_scale_kernel<false>, dim3(grad_blocks(chunks)), dim3(256), 0, (hipStream_t)stream, (const GradChunk*)table, chunks,
+                       (float*)clip, (const double*)nullptr, 0, 0.f);
     VINCE_CHECK_LAUNCH();
     return VINCE_OK;
 }
 
 extern "C" int vince_grad_clip(const void* table, int64_t chunks, float max_norm, float* clip, void* scratch, size_t scratch_bytes, void* stream) {
-    const int rc = vince_grad_norm(table, chunks, max_norm, clip, scratch, scratch_bytes, stream);
-    return rc != VINCE_OK ? rc : vince_grad_scale(table, chunks, clip, stream);
+    GRAD_NORM_CHECK("vince_grad_clip");
+    if (chunks == 0) return vince_grad_norm(table, chunks, max_norm, clip, scratch, scratch_bytes, stream);
+    const int blocks = grad_blocks(chunks);
+    hipLaunchKernelGGL(grad_squares_kernel, dim3(blocks), dim3(256), 0, (hipStream_t)stream, (const GradChunk*)table, chunks, (double*)scratch);
+    hipLaunchKernelGGL(grad_scale_kernel<true>, dim3(blocks), dim3(256), 0, (hipStream_t)stream, (const GradChunk*)table, chunks, clip,
+                       (const double*)scratch, blocks, max_norm);
+    VINCE_CHECK_LAUNCH();
+    return VINCE_OK;
 }
 
 extern "C" int vince_sgd_flat_clip(float* param, const float* grad, float* buf, int64_t n, float lr, float momentum, float weight_decay,

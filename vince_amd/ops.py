@@ -59,13 +59,19 @@ def _one_gpu(*tensors):
     return dev
 
 
+def _raw_stream(index):
+    """The current stream of device `index` as the C ABI takes it (0.1 us; through torch.cuda.current_stream() it is 2.7 us)."""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 def _launch(dev, fn, *args):
     """fn(*args, stream) on the current stream of `dev`, whichever device is current."""
-    if dev.index == torch.cuda.current_device():
-        check(fn(*args, torch.cuda.current_stream().cuda_stream))
+    index = dev.index
+    if index == torch.cuda.current_device():
+        check(fn(*args, _raw_stream(index)))
     else:
-        with torch.cuda.device(dev):
-            check(fn(*args, torch.cuda.current_stream().cuda_stream))
+        with torch.cuda.device(index):
+            check(fn(*args, _raw_stream(index)))
 
 
 # ------------------------------------------------------------------------------------------------ conv descriptors
@@ -819,20 +825,12 @@ class GradTable:
         check(lib().vince_grad_table_fill(entries, len(self.tensors), host.data_ptr(), self.chunks))
         self._table = host.to(self.device)            # (synchronous: any stream may read it from here on)
         self._scratch_bytes = lib().vince_grad_norm_scratch_bytes(self.chunks)
-        with torch.cuda.device(self.device):
-            self._stream = torch.cuda.current_stream().cuda_stream
+        self._stream = _raw_stream(self.device.index)
 
     def _run(self, fn, *args):
-        def go():
-            stream = torch.cuda.current_stream()
-            if stream.cuda_stream != self._stream:     # (its memory outlives what this stream still has to read)
-                self._table.record_stream(stream)
-            check(fn(self._table.data_ptr(), self.chunks, *args, stream.cuda_stream))
-        if self.device.index == torch.cuda.current_device():
-            go()
-        else:
-            with torch.cuda.device(self.device):
-                go()
+        if _raw_stream(self.device.index) != self._stream:     # (its memory outlives what another stream still has to read)
+            self._table.record_stream(torch.cuda.current_stream(self.device))
+        _launch(self.device, fn, self._table.data_ptr(), self.chunks, *args)
 
     def _norm(self, fn, max_norm):
         max_norm = float("inf") if max_norm is None else float(max_norm)
