@@ -1,106 +1,543 @@
 // Layer norm over the last axis of [rows][cols], forward and backward (include/vince_hip.h has the formulas).
-// One wavefront a row; the statistics are two-pass (the mean first, then the squares of the centred values), in fp32.
+//
+// Bound by HBM: the forward reads and writes every element once, the backward reads two (three with a ReLU) and writes one.  So a row
+// stays in registers from its one read to its write: TPR threads hold K 16-byte chunks each, the statistics are two-pass over the
+// registers (fp32; the mean first, then the squares of the centred values), and the next row's loads are in flight meanwhile.  Rows of
+// up to a wavefront's width take part of a wavefront, or one, with no barrier; longer ones a workgroup with one barrier a row.  Rows
+// past what a workgroup's registers hold are read again for every pass (the *_long kernels).
 #include "common.h"
 
 namespace {
 
-template <typename T> __device__ __forceinline__ float load1(const T* p) {
-    if constexpr (sizeof(T) == 4) return *p;
-    else return bf16_to_f32(*p);
+// ---- 16-byte chunks of a row at any element-aligned address ---------------------------------------------------------------------
+typedef __attribute__((ext_vector_type(4), aligned(2))) uint32_t u32x4_any_t;
+
+// n valid elements from p (whole chunks: one 16-byte load, whatever the alignment; the row's last: element by element), zeros behind
+template <typename T> __device__ __forceinline__ uint4 load_chunk(const T* __restrict__ p, int n) {
+    if (n >= Elem<T>::CH) {
+        const u32x4_any_t v = *(const u32x4_any_t*)p;
+        return make_uint4(v[0], v[1], v[2], v[3]);
+    }
+    uint32_t u[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int e = 0; e < Elem<T>::CH - 1; ++e)
+        if (e < n) {
+            if constexpr (sizeof(T) == 4) u[e] = __float_as_uint(p[e]);
+            else u[e >> 1] |= (uint32_t)p[e] << (16 * (e & 1));
+        }
+    return make_uint4(u[0], u[1], u[2], u[3]);
 }
-template <typename T> __device__ __forceinline__ void store1(T* p, float v) {
-    if constexpr (sizeof(T) == 4) *p = v;
-    else *p = f32_to_bf16(v);
+template <typename T> __device__ __forceinline__ void store_chunk(T* __restrict__ p, int n, const float* f) {
+    const uint4 q = Chunk<T>::pack(f);
+    if (n >= Elem<T>::CH) {
+        const u32x4_any_t v = {q.x, q.y, q.z, q.w};
+        *(u32x4_any_t*)p = v;
+        return;
+    }
+    const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int e = 0; e < Elem<T>::CH - 1; ++e)
+        if (e < n) {
+            if constexpr (sizeof(T) == 4) p[e] = __uint_as_float(u[e]);
+            else p[e] = (bf16_t)(u[e >> 1] >> (16 * (e & 1)));
+        }
+}
+// the same columns of an fp32 vector (NULL: `none` everywhere)
+template <int V> __device__ __forceinline__ void load_vector(const float* __restrict__ p, int64_t col, int n, float none, float* f) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) f[e] = p && e < n ? p[col + e] : none;
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void ln_fwd_kernel(const T* __restrict__ x, const float* __restrict__ w, const float* __restrict__ b,
-                                                     T* __restrict__ out, float* __restrict__ mean, float* __restrict__ rstd, int64_t rows,
-                                                     int cols, float eps, int relu) {
-    const int lane = threadIdx.x & 63;
-    for (int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); row < rows; row += (int64_t)gridDim.x * 4) {
-        const T* xr = x + row * cols;
-        T* yr = out + row * cols;
+// ---- sums over groups of lanes, every lane with the same bits ---------------------------------------------------------------------
+template <int CTRL> __device__ __forceinline__ float dpp(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+template <int N> __device__ __forceinline__ float lanes_sum(float v) {   // N = 2 .. 64 neighbouring lanes
+    if constexpr (N >= 2) v += dpp<0xB1>(v);       // quad_perm [1,0,3,2]
+    if constexpr (N >= 4) v += dpp<0x4E>(v);       // quad_perm [2,3,0,1]
+    if constexpr (N >= 8) v += dpp<0x141>(v);      // row_half_mirror
+    if constexpr (N >= 16) v += dpp<0x140>(v);     // row_mirror
+    if constexpr (N >= 32) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    if constexpr (N >= 64) {
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    return v;
+}
+
+constexpr int block_threads(int tpr) { return tpr > 256 ? tpr : 256; }
+
+// Where this thread's K chunks of a row are.  FULL: cols == TPR * K * V, every chunk whole.
+template <typename T, int TPR, int K, bool FULL> struct Cols {
+    static constexpr int V = Elem<T>::CH;
+    int lane, cols;
+    __device__ __forceinline__ Cols(int cols_) : lane((int)threadIdx.x % TPR), cols(cols_) {}
+    __device__ __forceinline__ int col(int k) const { return (k * TPR + lane) * V; }
+    __device__ __forceinline__ int valid(int k) const {   // elements of chunk k that are in the row
+        if constexpr (FULL) return V;
+        const int n = cols - col(k);
+        return n < 0 ? 0 : n > V ? V : n;
+    }
+    __device__ __forceinline__ void load(const T* __restrict__ row, uint4 (&q)[K]) const {
+#pragma unroll
+        for (int k = 0; k < K; ++k) q[k] = load_chunk<T>(row + col(k), valid(k));
+    }
+};
+
+template <typename T, int TPR, int K, bool FULL>
+__global__ __launch_bounds__(block_threads(TPR)) void ln_fwd_kernel(const T* __restrict__ x, const float* __restrict__ w,
+                                                                    const float* __restrict__ b, T* __restrict__ out, float* __restrict__ mean,
+                                                                    float* __restrict__ rstd, int64_t rows, int cols, float eps, int relu) {
+    constexpr int V = Elem<T>::CH, R = block_threads(TPR) / TPR, WAVES = TPR / 64;
+    const Cols<T, TPR, K, FULL> at(cols);
+    const float inv = 1.f / (float)cols;
+    __shared__ float2 part[2][WAVES > 1 ? WAVES : 1];    // mean and squares of each wavefront's columns, two rows' worth
+    float count = 0.f;                                    // elements of a row that this wavefront's (or group's) lanes hold
+#pragma unroll
+    for (int k = 0; k < K; ++k) count += (float)at.valid(k);
+    count = lanes_sum<(TPR < 64 ? TPR : 64)>(count);
+    if (FULL) count = (float)((TPR < 64 ? TPR : 64) * K * V);
+    __shared__ float counts[WAVES > 1 ? WAVES : 1];
+    if constexpr (WAVES > 1) {
+        if ((threadIdx.x & 63) == 0) counts[threadIdx.x >> 6] = count;
+        __syncthreads();
+    }
+    float wf[K][V], bf[K][V];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        load_vector<V>(w, at.col(k), at.valid(k), 1.f, wf[k]);
+        load_vector<V>(b, at.col(k), at.valid(k), 0.f, bf[k]);
+    }
+    const int64_t stride = (int64_t)gridDim.x * R;
+    int64_t row = (int64_t)blockIdx.x * R + threadIdx.x / TPR;
+    uint4 q[K];
+    if (row < rows) at.load(x + row * cols, q);
+    for (int turn = 0; row < rows; row += stride, turn ^= 1) {      // (a workgroup of one row leaves the loop as one: R == 1 with barriers)
+        float f[K][V];
+#pragma unroll
+        for (int k = 0; k < K; ++k) Chunk<T>::unpack(q[k], f[k]);
+        if (row + stride < rows) at.load(x + (row + stride) * cols, q);
         float s = 0.f;
-        for (int64_t i = lane; i < cols; i += 64) s += load1(xr + i);
-        const float m = wave_sum(s) / (float)cols;
-        float q = 0.f;
-        for (int64_t i = lane; i < cols; i += 64) { const float d = load1(xr + i) - m; q = fmaf(d, d, q); }
-        const float r = 1.f / sqrtf(wave_sum(q) / (float)cols + eps);
-        for (int64_t i = lane; i < cols; i += 64) {
-            float y = (load1(xr + i) - m) * r;
-            if (w) y = fmaf(y, w[i], b ? b[i] : 0.f);
-            if (relu && y < 0.f) y = 0.f;          // (a NaN stays)
-            store1(yr + i, y);
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int e = 0; e < V; ++e) s += f[k][e];
+        // means by division, not by a rounded reciprocal: a row of one value has exactly that mean, and its output is the bias
+        float m = lanes_sum<(TPR < 64 ? TPR : 64)>(s) / fmaxf(count, 1.f);
+        float ss = 0.f;
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const float d = FULL || e < at.valid(k) ? f[k][e] - m : 0.f;
+                ss = fmaf(d, d, ss);
+            }
+        ss = lanes_sum<(TPR < 64 ? TPR : 64)>(ss);
+        if constexpr (WAVES > 1) {       // the row's from the wavefronts': their squares about their own means, moved to the common one
+            if ((threadIdx.x & 63) == 0) part[turn][threadIdx.x >> 6] = make_float2(m, ss);
+            __syncthreads();             // (the other turn's slot is written only behind the next row's barrier: one barrier a row)
+            float2 p[WAVES];
+            m = 0.f;
+#pragma unroll
+            for (int i = 0; i < WAVES; ++i) {
+                p[i] = part[turn][i];
+                m = fmaf(p[i].x, FULL ? (float)(64 * K * V) : counts[i], m);
+            }
+            m /= (float)cols;
+            ss = 0.f;
+#pragma unroll
+            for (int i = 0; i < WAVES; ++i) {
+                const float d = p[i].x - m;
+                ss += fmaf(d * d, FULL ? (float)(64 * K * V) : counts[i], p[i].y);
+            }
         }
-        if (lane == 0) { mean[row] = m; rstd[row] = r; }
+        const float r = 1.f / sqrtf(fmaf(ss, inv, eps));
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            float y[V];
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                y[e] = fmaf((f[k][e] - m) * r, wf[k][e], bf[k][e]);
+                if (relu && y[e] < 0.f) y[e] = 0.f;          // (a NaN stays)
+            }
+            const int n = at.valid(k);
+            if (FULL || n > 0) store_chunk<T>(out + row * cols + at.col(k), n, y);
+        }
+        if (at.lane == 0) { mean[row] = m; rstd[row] = r; }
     }
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void ln_bwd_dx_kernel(const T* __restrict__ x, const float* __restrict__ w, const float* __restrict__ mean,
-                                                        const float* __restrict__ rstd, const T* __restrict__ dout, const T* __restrict__ act,
-                                                        T* __restrict__ dx, int64_t rows, int cols) {
-    const int lane = threadIdx.x & 63;
-    for (int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); row < rows; row += (int64_t)gridDim.x * 4) {
-        const int64_t at = row * cols;
-        const float m = mean[row], r = rstd[row];
+// ---- backward: dx, and this workgroup's sums for dweight and dbias ------------------------------------------------------------------
+// A thread has the same columns in every row it works on: its parts of dweight and dbias stay in registers until the last row.  Then the
+// R row groups of a workgroup are added up in LDS and one partial row [2][cols] a workgroup goes to scratch (or, with DIRECT, the only
+// workgroup writes the result).
+template <typename T, int TPR, int K, bool FULL>
+__global__ __launch_bounds__(block_threads(TPR)) void ln_bwd_kernel(const T* __restrict__ x, const float* __restrict__ w,
+                                                                    const float* __restrict__ mean, const float* __restrict__ rstd,
+                                                                    const T* __restrict__ dout, const T* __restrict__ act, T* __restrict__ dx,
+                                                                    float* __restrict__ dw_out, float* __restrict__ db_out, int accumulate,
+                                                                    float* __restrict__ partial, int64_t rows, int cols) {
+    constexpr int V = Elem<T>::CH, THREADS = block_threads(TPR), R = THREADS / TPR, WAVES = TPR / 64;
+    const Cols<T, TPR, K, FULL> at(cols);
+    const float inv = 1.f / (float)cols;
+    __shared__ float2 part[2][WAVES > 1 ? WAVES : 1];
+    float wf[K][V], dw[K][V], db[K][V];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        load_vector<V>(w, at.col(k), at.valid(k), 1.f, wf[k]);
+#pragma unroll
+        for (int e = 0; e < V; ++e) dw[k][e] = db[k][e] = 0.f;
+    }
+    const int64_t stride = (int64_t)gridDim.x * R;
+    int64_t row = (int64_t)blockIdx.x * R + threadIdx.x / TPR;
+    uint4 qx[K], qd[K], qa[K];
+    float m_next = 0.f, r_next = 0.f;
+    auto fetch = [&](int64_t i) {
+        at.load(x + i * cols, qx);
+        at.load(dout + i * cols, qd);
+        if (act) at.load(act + i * cols, qa);
+        m_next = mean[i];
+        r_next = rstd[i];
+    };
+    if (row < rows) fetch(row);
+    for (int turn = 0; row < rows; row += stride, turn ^= 1) {
+        float xh[K][V], g[K][V];
+        const float m = m_next, r = r_next;
         float c1 = 0.f, c2 = 0.f;
-        for (int64_t i = lane; i < cols; i += 64) {
-            float g = load1(dout + at + i);
-            if (act && !(load1(act + at + i) > 0.f)) g = 0.f;
-            if (w) g *= w[i];
-            c1 += g;
-            c2 = fmaf(g, (load1(x + at + i) - m) * r, c2);
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            Chunk<T>::unpack(qx[k], xh[k]);
+            Chunk<T>::unpack(qd[k], g[k]);
+            if (act) {
+                float a[V];
+                Chunk<T>::unpack(qa[k], a);
+#pragma unroll
+                for (int e = 0; e < V; ++e) g[k][e] = a[e] > 0.f ? g[k][e] : 0.f;
+            }
         }
-        c1 = wave_sum(c1) / (float)cols;
-        c2 = wave_sum(c2) / (float)cols;
-        for (int64_t i = lane; i < cols; i += 64) {
-            float g = load1(dout + at + i);
-            if (act && !(load1(act + at + i) > 0.f)) g = 0.f;
-            if (w) g *= w[i];
-            store1(dx + at + i, r * (g - c1 - (load1(x + at + i) - m) * r * c2));
+        if (row + stride < rows) fetch(row + stride);
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                xh[k][e] = FULL || e < at.valid(k) ? (xh[k][e] - m) * r : 0.f;
+                db[k][e] += g[k][e];
+                dw[k][e] = fmaf(g[k][e], xh[k][e], dw[k][e]);
+                g[k][e] *= wf[k][e];
+                c1 += g[k][e];
+                c2 = fmaf(g[k][e], xh[k][e], c2);
+            }
+        c1 = lanes_sum<(TPR < 64 ? TPR : 64)>(c1);
+        c2 = lanes_sum<(TPR < 64 ? TPR : 64)>(c2);
+        if constexpr (WAVES > 1) {
+            if ((threadIdx.x & 63) == 0) part[turn][threadIdx.x >> 6] = make_float2(c1, c2);
+            __syncthreads();
+            c1 = c2 = 0.f;
+#pragma unroll
+            for (int i = 0; i < WAVES; ++i) { c1 += part[turn][i].x; c2 += part[turn][i].y; }
+        }
+        c1 *= inv;
+        c2 *= inv;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            float y[V];
+#pragma unroll
+            for (int e = 0; e < V; ++e) y[e] = r * (g[k][e] - c1 - xh[k][e] * c2);
+            const int n = at.valid(k);
+            if (FULL || n > 0) store_chunk<T>(dx + row * cols + at.col(k), n, y);
+        }
+    }
+    if (!dw_out) return;
+    // one row group a workgroup: the registers are the workgroup's sums; several: added up in LDS in the order of the groups
+    __shared__ float red[R > 1 ? THREADS * K * V : 1];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        float(&v)[K][V] = half == 0 ? dw : db;
+        if constexpr (R > 1) {
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int e = 0; e < V; ++e) red[(threadIdx.x / TPR * K + k) * (TPR * V) + at.lane * V + e] = v[k][e];
+            __syncthreads();
+        }
+        float* final_out = half == 0 ? dw_out : db_out;
+        float* to = partial ? partial + ((int64_t)blockIdx.x * 2 + half) * cols : final_out;
+        const bool add = !partial && accumulate;
+        if constexpr (R > 1) {
+            for (int c = threadIdx.x; c < cols; c += THREADS) {       // (cols <= TPR * K * V)
+                float s = 0.f;
+#pragma unroll 8
+                for (int i = 0; i < R; ++i) s += red[i * (K * TPR * V) + c];
+                to[c] = add ? to[c] + s : s;
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+#pragma unroll
+                for (int e = 0; e < V; ++e)
+                    if (FULL || e < at.valid(k)) {
+                        const int c = at.col(k) + e;
+                        to[c] = add ? to[c] + v[k][e] : v[k][e];
+                    }
         }
     }
 }
 
-// sums over the rows [y * per, (y + 1) * per) of 64 columns: partial [part][2][cols]
-template <typename T>
-__global__ __launch_bounds__(256) void ln_bwd_dw_kernel(const T* __restrict__ x, const float* __restrict__ mean, const float* __restrict__ rstd,
-                                                        const T* __restrict__ dout, const T* __restrict__ act, float* __restrict__ partial,
-                                                        int64_t rows, int cols, int64_t per) {
-    __shared__ float red[2][4][64];
-    const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
-    const int64_t c = (int64_t)blockIdx.x * 64 + tx;
-    const int64_t r0 = (int64_t)blockIdx.y * per, r1 = r0 + per < rows ? r0 + per : rows;
-    float dw = 0.f, db = 0.f;
-    if (c < cols)
-        for (int64_t row = r0 + ty; row < r1; row += 4) {
-            const int64_t i = row * cols + c;
-            float g = load1(dout + i);
-            if (act && !(load1(act + i) > 0.f)) g = 0.f;
-            db += g;
-            dw = fmaf(g, (load1(x + i) - mean[row]) * rstd[row], dw);
+// dweight / dbias = (or +=) the sum of `parts` partial rows [2][cols]: 32 columns x 32 rows at a time, the rows' sums in a fixed order
+__global__ __launch_bounds__(1024) void ln_bwd_join_kernel(const float* __restrict__ partial, int parts, int64_t cols2, int cols,
+                                                           float* __restrict__ dw, float* __restrict__ db, int accumulate) {
+    __shared__ float red[32][33];
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    const int64_t c = (int64_t)blockIdx.x * 32 + tx;
+    float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+    if (c < cols2) {
+        const float* p = partial + c;
+        int i = ty;
+        for (; i + 96 < parts; i += 128) {
+            const float a0 = p[(int64_t)i * cols2], a1 = p[(int64_t)(i + 32) * cols2], a2 = p[(int64_t)(i + 64) * cols2],
+                        a3 = p[(int64_t)(i + 96) * cols2];
+            s0 += a0; s1 += a1; s2 += a2; s3 += a3;
         }
-    red[0][ty][tx] = dw;
-    red[1][ty][tx] = db;
+        for (; i < parts; i += 32) s0 += p[(int64_t)i * cols2];
+    }
+    red[ty][tx] = (s0 + s1) + (s2 + s3);
     __syncthreads();
-    if (ty < 2 && c < cols)
-        partial[((int64_t)blockIdx.y * 2 + ty) * cols + c] = red[ty][0][tx] + red[ty][1][tx] + red[ty][2][tx] + red[ty][3][tx];
+    if (ty == 0 && c < cols2) {
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) s += red[i][tx];
+        float* out = c < cols ? dw + c : db + (c - cols);
+        *out = accumulate ? *out + s : s;
+    }
 }
 
-// dweight / dbias = (or +=) the sum of the partials in the order of their rows
-__global__ __launch_bounds__(256) void ln_bwd_join_kernel(const float* __restrict__ partial, int parts, int cols, float* __restrict__ dw,
-                                                          float* __restrict__ db, int accumulate) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= 2 * (int64_t)cols) return;
-    float* out = i < cols ? dw + i : db + (i - cols);
+// ---- rows longer than a workgroup's registers -----------------------------------------------------------------------------------------
+template <int WAVES> __device__ __forceinline__ float block_sum(float v, float* red) {
+    v = lanes_sum<64>(v);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
     float s = 0.f;
-    for (int p = 0; p < parts; ++p) s += partial[(int64_t)p * 2 * cols + i];
-    *out = accumulate ? *out + s : s;
+#pragma unroll
+    for (int i = 0; i < WAVES; ++i) s += red[i];
+    return s;
 }
 
-int ln_parts(int64_t rows) { return (int)(rows < 64 ? 1 : rows < 64 * 128 ? rows / 64 : 128); }
+template <typename T>
+__global__ __launch_bounds__(1024) void ln_fwd_long_kernel(const T* __restrict__ x, const float* __restrict__ w, const float* __restrict__ b,
+                                                           T* __restrict__ out, float* __restrict__ mean, float* __restrict__ rstd, int64_t rows,
+                                                           int cols, float eps, int relu) {
+    constexpr int V = Elem<T>::CH;
+    __shared__ float red[16];
+    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+        const T* xr = x + row * cols;
+        float s = 0.f, f[V];
+        for (int64_t c = threadIdx.x * V; c < cols; c += 1024 * V) {
+            Chunk<T>::unpack(load_chunk<T>(xr + c, cols - c < V ? (int)(cols - c) : V), f);
+#pragma unroll
+            for (int e = 0; e < V; ++e) s += f[e];
+        }
+        const float m = block_sum<16>(s, red) / (float)cols;
+        s = 0.f;
+        for (int64_t c = threadIdx.x * V; c < cols; c += 1024 * V) {
+            const int n = cols - c < V ? (int)(cols - c) : V;
+            Chunk<T>::unpack(load_chunk<T>(xr + c, n), f);
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const float d = e < n ? f[e] - m : 0.f;
+                s = fmaf(d, d, s);
+            }
+        }
+        const float r = 1.f / sqrtf(block_sum<16>(s, red) / (float)cols + eps);
+        for (int64_t c = threadIdx.x * V; c < cols; c += 1024 * V) {
+            const int n = cols - c < V ? (int)(cols - c) : V;
+            float wf[V], bf[V];
+            Chunk<T>::unpack(load_chunk<T>(xr + c, n), f);
+            load_vector<V>(w, c, n, 1.f, wf);
+            load_vector<V>(b, c, n, 0.f, bf);
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                f[e] = fmaf((f[e] - m) * r, wf[e], bf[e]);
+                if (relu && f[e] < 0.f) f[e] = 0.f;
+            }
+            store_chunk<T>(out + row * cols + c, n, f);
+        }
+        if (threadIdx.x == 0) { mean[row] = m; rstd[row] = r; }
+    }
+}
+
+// d (masked) and xhat of one chunk
+template <typename T>
+__device__ __forceinline__ void grad_chunk(const T* __restrict__ x, const T* __restrict__ dout, const T* __restrict__ act, int64_t i, int n, float m,
+                                           float r, float* d, float* xh) {
+    constexpr int V = Elem<T>::CH;
+    Chunk<T>::unpack(load_chunk<T>(x + i, n), xh);
+    Chunk<T>::unpack(load_chunk<T>(dout + i, n), d);
+    if (act) {
+        float a[V];
+        Chunk<T>::unpack(load_chunk<T>(act + i, n), a);
+#pragma unroll
+        for (int e = 0; e < V; ++e) d[e] = a[e] > 0.f ? d[e] : 0.f;
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e) xh[e] = e < n ? (xh[e] - m) * r : 0.f;
+}
+
+template <typename T>
+__global__ __launch_bounds__(1024) void ln_bwd_long_dx_kernel(const T* __restrict__ x, const float* __restrict__ w, const float* __restrict__ mean,
+                                                              const float* __restrict__ rstd, const T* __restrict__ dout,
+                                                              const T* __restrict__ act, T* __restrict__ dx, int64_t rows, int cols) {
+    constexpr int V = Elem<T>::CH;
+    __shared__ float red[16];
+    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+        const float m = mean[row], r = rstd[row];
+        float c1 = 0.f, c2 = 0.f, d[V], xh[V], wf[V];
+        for (int64_t c = threadIdx.x * V; c < cols; c += 1024 * V) {
+            const int n = cols - c < V ? (int)(cols - c) : V;
+            grad_chunk<T>(x, dout, act, row * cols + c, n, m, r, d, xh);
+            load_vector<V>(w, c, n, 1.f, wf);
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const float g = d[e] * wf[e];
+                c1 += g;
+                c2 = fmaf(g, xh[e], c2);
+            }
+        }
+        c1 = block_sum<16>(c1, red) / (float)cols;
+        c2 = block_sum<16>(c2, red) / (float)cols;
+        for (int64_t c = threadIdx.x * V; c < cols; c += 1024 * V) {
+            const int n = cols - c < V ? (int)(cols - c) : V;
+            grad_chunk<T>(x, dout, act, row * cols + c, n, m, r, d, xh);
+            load_vector<V>(w, c, n, 1.f, wf);
+#pragma unroll
+            for (int e = 0; e < V; ++e) d[e] = r * (d[e] * wf[e] - c1 - xh[e] * c2);
+            store_chunk<T>(dx + row * cols + c, n, d);
+        }
+    }
+}
+
+// partial sums over the rows blockIdx.y, blockIdx.y + gridDim.y, ... of one chunk of columns a thread
+template <typename T>
+__global__ __launch_bounds__(256) void ln_bwd_long_dw_kernel(const T* __restrict__ x, const float* __restrict__ mean, const float* __restrict__ rstd,
+                                                             const T* __restrict__ dout, const T* __restrict__ act, float* __restrict__ partial,
+                                                             int64_t rows, int cols) {
+    constexpr int V = Elem<T>::CH;
+    const int64_t c = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V;
+    if (c >= cols) return;
+    const int n = cols - c < V ? (int)(cols - c) : V;
+    float dw[V], db[V], d[V], xh[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) dw[e] = db[e] = 0.f;
+#pragma unroll 4
+    for (int64_t row = blockIdx.y; row < rows; row += gridDim.y) {
+        grad_chunk<T>(x, dout, act, row * cols + c, n, mean[row], rstd[row], d, xh);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            db[e] += d[e];
+            dw[e] = fmaf(d[e], xh[e], dw[e]);
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+        if (e < n) {
+            partial[((int64_t)blockIdx.y * 2) * cols + c + e] = dw[e];
+            partial[((int64_t)blockIdx.y * 2 + 1) * cols + c + e] = db[e];
+        }
+}
+
+// ---- which split -----------------------------------------------------------------------------------------------------------------------
+// Threads a row and chunks a thread, from the row's number of 16-byte chunks.  Up to 64 chunks: one a lane, the smallest power of two of
+// lanes (several rows share a wavefront).  Then a wavefront with up to KMAX a lane, then a workgroup of 256 .. 1024.  KMAX: what the
+// registers hold with four wavefronts a SIMD -- 4 forward; backward, which keeps a weight and two sums a column, 16 values (4 fp32
+// chunks, 2 bf16).
+struct Split { int tpr, k; };
+Split ln_split(int64_t chunks, int kmax) {
+    if (chunks <= 64) {
+        int tpr = 2;
+        while (tpr < chunks) tpr *= 2;
+        return {tpr, 1};
+    }
+    for (int tpr = 64; tpr <= 1024; tpr = tpr == 64 ? 256 : tpr * 2)
+        for (int k = 1; k <= kmax; k *= 2)
+            if ((int64_t)tpr * k >= chunks) return {tpr, k};
+    return {0, 0};
+}
+int ln_chunks(int dtype, int cols) { const int v = dtype == VINCE_F32 ? 4 : 8; return (cols + v - 1) / v; }
+constexpr int LN_FWD_K = 4;
+constexpr int ln_bwd_k(int dtype) { return dtype == VINCE_F32 ? 4 : 2; }
+
+// Workgroups of the backward: at most two a CU -- each writes a partial row of 8 bytes a column that is read again -- and at least four
+// rows for each row group, so that the partial rows stay a small part of what is read anyway.
+int ln_bwd_blocks(int64_t rows, const Split& s) {
+    const int64_t per = s.tpr == 0 ? 4 : 4 * (block_threads(s.tpr) / s.tpr);
+    const int64_t n = (rows + per - 1) / per;
+    return (int)(n < 1 ? 1 : n > 512 ? 512 : n);
+}
+
+template <typename T, int TPR, int K>
+void launch_fwd(const void* x, const float* w, const float* b, void* out, float* mean, float* rstd, int64_t rows, int cols, float eps, int relu,
+                hipStream_t st) {
+    constexpr int THREADS = block_threads(TPR), R = THREADS / TPR;
+    const int64_t want = (rows + R - 1) / R, most = 256 * 2048 / THREADS;
+    const dim3 grid((unsigned)(want < most ? want : most));
+    if (cols == TPR * K * Elem<T>::CH)
+        hipLaunchKernelGGL((ln_fwd_kernel<T, TPR, K, true>), grid, dim3(THREADS), 0, st, (const T*)x, w, b, (T*)out, mean, rstd, rows, cols, eps, relu);
+    else
+        hipLaunchKernelGGL((ln_fwd_kernel<T, TPR, K, false>), grid, dim3(THREADS), 0, st, (const T*)x, w, b, (T*)out, mean, rstd, rows, cols, eps, relu);
+}
+
+template <typename T>
+void run_fwd(int dtype, const void* x, const float* w, const float* b, void* out, float* mean, float* rstd, int64_t rows, int cols, float eps,
+             int relu, hipStream_t st) {
+    const Split s = ln_split(ln_chunks(dtype, cols), LN_FWD_K);
+#define LN_CASE(TPR, K) \
+    if (s.tpr == TPR && s.k == K) return launch_fwd<T, TPR, K>(x, w, b, out, mean, rstd, rows, cols, eps, relu, st)
+    LN_CASE(2, 1); LN_CASE(4, 1); LN_CASE(8, 1); LN_CASE(16, 1); LN_CASE(32, 1); LN_CASE(64, 1); LN_CASE(64, 2); LN_CASE(64, 4);
+    LN_CASE(256, 2); LN_CASE(256, 4); LN_CASE(512, 4); LN_CASE(1024, 4);
+#undef LN_CASE
+    hipLaunchKernelGGL(ln_fwd_long_kernel<T>, dim3((unsigned)(rows < 1024 ? rows : 1024)), dim3(1024), 0, st, (const T*)x, w, b, (T*)out, mean, rstd,
+                       rows, cols, eps, relu);
+}
+
+struct BwdArgs {
+    const void *x, *dout, *act;
+    const float *w, *mean, *rstd;
+    void* dx;
+    float *dw, *db, *partial;
+    int accumulate;
+    int64_t rows;
+    int cols, blocks;
+};
+
+template <typename T, int TPR, int K> void launch_bwd(const BwdArgs& a, hipStream_t st) {
+    if (a.cols == TPR * K * Elem<T>::CH)
+        hipLaunchKernelGGL((ln_bwd_kernel<T, TPR, K, true>), dim3(a.blocks), dim3(block_threads(TPR)), 0, st, (const T*)a.x, a.w, a.mean, a.rstd,
+                           (const T*)a.dout, (const T*)a.act, (T*)a.dx, a.dw, a.db, a.accumulate, a.partial, a.rows, a.cols);
+    else
+        hipLaunchKernelGGL((ln_bwd_kernel<T, TPR, K, false>), dim3(a.blocks), dim3(block_threads(TPR)), 0, st, (const T*)a.x, a.w, a.mean, a.rstd,
+                           (const T*)a.dout, (const T*)a.act, (T*)a.dx, a.dw, a.db, a.accumulate, a.partial, a.rows, a.cols);
+}
+
+template <typename T> void run_bwd(const Split& s, const BwdArgs& a, hipStream_t st) {
+#define LN_CASE(TPR, K) \
+    if (s.tpr == TPR && s.k == K) return launch_bwd<T, TPR, K>(a, st)
+    LN_CASE(2, 1); LN_CASE(4, 1); LN_CASE(8, 1); LN_CASE(16, 1); LN_CASE(32, 1); LN_CASE(64, 1); LN_CASE(64, 2); LN_CASE(256, 2);
+    if constexpr (sizeof(T) == 4) {
+        LN_CASE(64, 4); LN_CASE(256, 4); LN_CASE(512, 4); LN_CASE(1024, 4);
+    } else {
+        LN_CASE(256, 1); LN_CASE(512, 2); LN_CASE(1024, 2);
+    }
+#undef LN_CASE
+    hipLaunchKernelGGL(ln_bwd_long_dx_kernel<T>, dim3((unsigned)(a.rows < 1024 ? a.rows : 1024)), dim3(1024), 0, st, (const T*)a.x, a.w, a.mean,
+                       a.rstd, (const T*)a.dout, (const T*)a.act, (T*)a.dx, a.rows, a.cols);
+    if (a.dw)
+        hipLaunchKernelGGL(ln_bwd_long_dw_kernel<T>, dim3((unsigned)((a.cols + 256 * Elem<T>::CH - 1) / (256 * Elem<T>::CH)), (unsigned)a.blocks),
+                           dim3(256), 0, st, (const T*)a.x, a.mean, a.rstd, (const T*)a.dout, (const T*)a.act, a.partial, a.rows, a.cols);
+}
 
 }  // namespace
 
@@ -114,21 +551,17 @@ extern "C" int vince_layer_norm_fwd(int dtype, const void* x, const float* weigh
     VINCE_CHECK_ARG(eps >= 0.f, VINCE_E_ARG, "vince_layer_norm_fwd: eps=%g", (double)eps);
     if (rows == 0) return VINCE_OK;
     VINCE_CHECK_ARG(x && out && mean && rstd && (weight || !bias), VINCE_E_ARG, "vince_layer_norm_fwd: null pointer, or a bias without a weight");
-    const dim3 grid((unsigned)((rows + 3) / 4 < 65536 ? (rows + 3) / 4 : 65536));
-    if (dtype == VINCE_F32)
-        hipLaunchKernelGGL(ln_fwd_kernel<float>, grid, dim3(256), 0, (hipStream_t)stream, (const float*)x, weight, bias, (float*)out, mean, rstd,
-                           rows, cols, eps, relu);
-    else
-        hipLaunchKernelGGL(ln_fwd_kernel<bf16_t>, grid, dim3(256), 0, (hipStream_t)stream, (const bf16_t*)x, weight, bias, (bf16_t*)out, mean,
-                           rstd, rows, cols, eps, relu);
+    if (dtype == VINCE_F32) run_fwd<float>(dtype, x, weight, bias, out, mean, rstd, rows, cols, eps, relu, (hipStream_t)stream);
+    else run_fwd<bf16_t>(dtype, x, weight, bias, out, mean, rstd, rows, cols, eps, relu, (hipStream_t)stream);
     VINCE_CHECK_LAUNCH();
     return VINCE_OK;
 }
 
 extern "C" size_t vince_layer_norm_bwd_scratch_bytes(int dtype, int64_t rows, int32_t cols) {
-    (void)dtype;
     if (rows <= 0 || cols <= 0) return 0;
-    return (size_t)ln_parts(rows) * 2 * (size_t)cols * sizeof(float);
+    const Split s = ln_split(ln_chunks(dtype, cols), ln_bwd_k(dtype));
+    const int blocks = ln_bwd_blocks(rows, s);
+    return blocks == 1 && s.tpr ? 0 : (size_t)blocks * 2 * (size_t)cols * sizeof(float);
 }
 
 extern "C" int vince_layer_norm_bwd(int dtype, const void* x, const float* weight, const float* mean, const float* rstd, const void* dout,
@@ -137,32 +570,21 @@ extern "C" int vince_layer_norm_bwd(int dtype, const void* x, const float* weigh
     LN_CHECK("vince_layer_norm_bwd");
     VINCE_CHECK_ARG((dweight == nullptr) == (dbias == nullptr), VINCE_E_ARG, "vince_layer_norm_bwd: dweight and dbias come together");
     hipStream_t st = (hipStream_t)stream;
+    const Split s = ln_split(ln_chunks(dtype, cols), ln_bwd_k(dtype));
+    const int blocks = ln_bwd_blocks(rows, s);
+    const bool direct = rows > 0 && blocks == 1 && s.tpr;       // one workgroup: it writes dweight and dbias itself
     if (rows > 0) {
         VINCE_CHECK_ARG(x && mean && rstd && dout && dx, VINCE_E_ARG, "vince_layer_norm_bwd: null pointer");
-        VINCE_CHECK_ARG(!dweight || (scratch && scratch_bytes >= vince_layer_norm_bwd_scratch_bytes(dtype, rows, cols)), VINCE_E_ARG,
-                        "vince_layer_norm_bwd: scratch of %zu bytes", scratch_bytes);
-        const dim3 grid((unsigned)((rows + 3) / 4 < 65536 ? (rows + 3) / 4 : 65536));
-        const int parts = ln_parts(rows);
-        const dim3 grid2((unsigned)((cols + 63) / 64), parts);
-        const int64_t per = (rows + parts - 1) / parts;
-        if (dtype == VINCE_F32) {
-            hipLaunchKernelGGL(ln_bwd_dx_kernel<float>, grid, dim3(256), 0, st, (const float*)x, weight, mean, rstd, (const float*)dout,
-                               (const float*)act, (float*)dx, rows, cols);
-            if (dweight)
-                hipLaunchKernelGGL(ln_bwd_dw_kernel<float>, grid2, dim3(256), 0, st, (const float*)x, mean, rstd, (const float*)dout,
-                                   (const float*)act, (float*)scratch, rows, cols, per);
-        } else {
-            hipLaunchKernelGGL(ln_bwd_dx_kernel<bf16_t>, grid, dim3(256), 0, st, (const bf16_t*)x, weight, mean, rstd, (const bf16_t*)dout,
-                               (const bf16_t*)act, (bf16_t*)dx, rows, cols);
-            if (dweight)
-                hipLaunchKernelGGL(ln_bwd_dw_kernel<bf16_t>, grid2, dim3(256), 0, st, (const bf16_t*)x, mean, rstd, (const bf16_t*)dout,
-                                   (const bf16_t*)act, (float*)scratch, rows, cols, per);
-        }
+        const size_t need = dweight ? vince_layer_norm_bwd_scratch_bytes(dtype, rows, cols) : 0;
+        VINCE_CHECK_ARG(need == 0 || (scratch && scratch_bytes >= need), VINCE_E_ARG, "vince_layer_norm_bwd: scratch of %zu bytes", scratch_bytes);
+        const BwdArgs a = {x, dout, act, weight, mean, rstd, dx, dweight, dbias, direct ? nullptr : (float*)scratch, accumulate, rows, cols, blocks};
+        if (dtype == VINCE_F32) run_bwd<float>(s, a, st);
+        else run_bwd<bf16_t>(s, a, st);
         VINCE_CHECK_LAUNCH();
     }
-    if (dweight && (rows > 0 || !accumulate)) {
-        hipLaunchKernelGGL(ln_bwd_join_kernel, dim3((unsigned)((2 * (int64_t)cols + 255) / 256)), dim3(256), 0, st, (const float*)scratch,
-                           rows > 0 ? ln_parts(rows) : 0, cols, dweight, dbias, accumulate);
+    if (dweight && !direct && (rows > 0 || !accumulate)) {
+        hipLaunchKernelGGL(ln_bwd_join_kernel, dim3((unsigned)((2 * (int64_t)cols + 31) / 32)), dim3(1024), 0, st, (const float*)scratch,
+                           rows > 0 ? blocks : 0, 2 * (int64_t)cols, cols, dweight, dbias, accumulate);
         VINCE_CHECK_LAUNCH();
     }
     return VINCE_OK;
