@@ -12,40 +12,78 @@ namespace {
 // ---- 16-byte chunks of a row at any element-aligned address ---------------------------------------------------------------------
 typedef __attribute__((ext_vector_type(4), aligned(2))) uint32_t u32x4_any_t;
 
-// n valid elements from p (whole chunks: one 16-byte load, whatever the alignment; the row's last: element by element), zeros behind
-template <typename T> __device__ __forceinline__ uint4 load_chunk(const T* __restrict__ p, int n) {
-    if (n >= Elem<T>::CH) {
-        const u32x4_any_t v = *(const u32x4_any_t*)p;
-        return make_uint4(v[0], v[1], v[2], v[3]);
-    }
-    uint32_t u[4] = {0u, 0u, 0u, 0u};
-#pragma unroll
-    for (int e = 0; e < Elem<T>::CH - 1; ++e)
-        if (e < n) {
-            if constexpr (sizeof(T) == 4) u[e] = __float_as_uint(p[e]);
-            else u[e >> 1] |= (uint32_t)p[e] << (16 * (e & 1));
-        }
-    return make_uint4(u[0], u[1], u[2], u[3]);
+template <typename T> __device__ __forceinline__ uint4 load16(const T* __restrict__ p) {
+    const u32x4_any_t v = *(const u32x4_any_t*)p;
+    return make_uint4(v[0], v[1], v[2], v[3]);
 }
+// The chunk at column `col` of a row, zeros behind the row's end.  One load whatever the chunk holds: a chunk that the row's end cuts
+// is read as the row's last 16 bytes and shifted down (element by element it would be seven loads, or seven round trips).
+template <typename T, bool FULL, typename I> __device__ __forceinline__ uint4 load_chunk(const T* __restrict__ row, I col, I cols) {
+    constexpr int V = Elem<T>::CH, BITS = 8 * sizeof(T);
+    if constexpr (FULL) return load16<T>(row + col);
+    if (cols < V) {                                       // (a row of less than 16 bytes; uniform)
+        uint32_t u[4] = {0u, 0u, 0u, 0u};
+        if (col == 0)
+#pragma unroll
+            for (int e = 0; e < V - 1; ++e) {
+                const T one = row[e < cols ? e : 0];
+                uint32_t bits;
+                if constexpr (sizeof(T) == 4) bits = __float_as_uint(one);
+                else bits = one;
+                if (e < cols) u[e * sizeof(T) / 4] |= bits << (e * BITS % 32);
+            }
+        return make_uint4(u[0], u[1], u[2], u[3]);
+    }
+    const I last = cols - V, from = col < last ? col : last;
+    uint4 q = load16<T>(row + from);
+    if (col > last) {
+        const int shift = (int)(col - last < V ? col - last : V) * BITS;       // 128: nothing of the chunk is in the row
+        unsigned __int128 v = ((unsigned __int128)(((uint64_t)q.w << 32) | q.z) << 64) | (((uint64_t)q.y << 32) | q.x);
+        v = shift >= 128 ? 0 : v >> shift;
+        q = make_uint4((uint32_t)v, (uint32_t)(v >> 32), (uint32_t)(v >> 64), (uint32_t)(v >> 96));
+    }
+    return q;
+}
+// n elements of a chunk to p: whole, or the 4 / 2 / 1 elements that n is made of
 template <typename T> __device__ __forceinline__ void store_chunk(T* __restrict__ p, int n, const float* f) {
+    typedef __attribute__((ext_vector_type(2), aligned(2))) uint32_t u32x2_any_t;
+    typedef __attribute__((aligned(2))) uint32_t u32_any_t;
+    constexpr int V = Elem<T>::CH;
     const uint4 q = Chunk<T>::pack(f);
-    if (n >= Elem<T>::CH) {
+    if (n >= V) {
         const u32x4_any_t v = {q.x, q.y, q.z, q.w};
         *(u32x4_any_t*)p = v;
         return;
     }
-    const uint32_t u[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-    for (int e = 0; e < Elem<T>::CH - 1; ++e)
-        if (e < n) {
-            if constexpr (sizeof(T) == 4) p[e] = __uint_as_float(u[e]);
-            else p[e] = (bf16_t)(u[e >> 1] >> (16 * (e & 1)));
+    uint32_t a = q.x, b = q.y, c = q.z;
+    if (n & (V / 2)) {
+        const u32x2_any_t v = {a, b};
+        *(u32x2_any_t*)p = v;
+        p += V / 2;
+        a = c;
+        b = q.w;
+    }
+    if constexpr (sizeof(T) == 2) {
+        if (n & 2) {
+            *(u32_any_t*)p = a;
+            p += 2;
+            a = b;
         }
+    }
+    if (n & 1) {
+        if constexpr (sizeof(T) == 4) *p = __uint_as_float(a);
+        else *p = (bf16_t)a;
+    }
 }
 // the same columns of an fp32 vector (NULL: `none` everywhere)
-template <int V> __device__ __forceinline__ void load_vector(const float* __restrict__ p, int64_t col, int n, float none, float* f) {
+template <int V, bool FULL, typename I> __device__ __forceinline__ void load_vector(const float* __restrict__ p, I col, I cols, float none, float* f) {
+    if (!p) {
 #pragma unroll
-    for (int e = 0; e < V; ++e) f[e] = p && e < n ? p[col + e] : none;
+        for (int e = 0; e < V; ++e) f[e] = none;
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < V; e += 4) Chunk<float>::unpack(load_chunk<float, FULL>(p, (I)(col + e), cols), f + e);
 }
 
 // ---- sums over groups of lanes, every lane with the same bits ---------------------------------------------------------------------
@@ -69,21 +107,30 @@ template <int N> __device__ __forceinline__ float lanes_sum(float v) {   // N = 
 }
 
 constexpr int block_threads(int tpr) { return tpr > 256 ? tpr : 256; }
+// Whether a thread keeps its columns' weight (and bias) in registers from row to row.  At 1024 threads, with 128 registers each, there is
+// no room: they are read again for every row, from the caches.
+constexpr bool holds_weights(int tpr) { return tpr < 1024; }
 
-// Where this thread's K chunks of a row are.  FULL: cols == TPR * K * V, every chunk whole.
+// Where this thread's K chunks of a row are.  FULL: cols == TPR * K * V, every chunk whole.  Else the first K / 2 are (ln_split takes K > 1
+// for rows of more than TPR * K / 2 chunks), the others may be cut by the row's end or lie behind it.
 template <typename T, int TPR, int K, bool FULL> struct Cols {
     static constexpr int V = Elem<T>::CH;
     int lane, cols;
     __device__ __forceinline__ Cols(int cols_) : lane((int)threadIdx.x % TPR), cols(cols_) {}
     __device__ __forceinline__ int col(int k) const { return (k * TPR + lane) * V; }
+    static constexpr bool whole(int k) { return FULL || k < K / 2; }
     __device__ __forceinline__ int valid(int k) const {   // elements of chunk k that are in the row
-        if constexpr (FULL) return V;
+        if (whole(k)) return V;
         const int n = cols - col(k);
         return n < 0 ? 0 : n > V ? V : n;
     }
     __device__ __forceinline__ void load(const T* __restrict__ row, uint4 (&q)[K]) const {
 #pragma unroll
-        for (int k = 0; k < K; ++k) q[k] = load_chunk<T>(row + col(k), valid(k));
+        for (int k = 0; k < K; ++k) q[k] = whole(k) ? load_chunk<T, true>(row, col(k), cols) : load_chunk<T, false>(row, col(k), cols);
+    }
+    __device__ __forceinline__ void load(const float* __restrict__ p, float none, int k, float (&f)[V]) const {   // of a vector of the row's length
+        if (whole(k)) load_vector<V, true>(p, col(k), cols, none, f);
+        else load_vector<V, false>(p, col(k), cols, none, f);
     }
 };
 
@@ -105,17 +152,22 @@ __global__ __launch_bounds__(block_threads(TPR)) void ln_fwd_kernel(const T* __r
         if ((threadIdx.x & 63) == 0) counts[threadIdx.x >> 6] = count;
         __syncthreads();
     }
-    float wf[K][V], bf[K][V];
+    constexpr bool HOLD = holds_weights(TPR);
+    float wf[HOLD ? K : 1][V], bf[HOLD ? K : 1][V];
+    if constexpr (HOLD) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-        load_vector<V>(w, at.col(k), at.valid(k), 1.f, wf[k]);
-        load_vector<V>(b, at.col(k), at.valid(k), 0.f, bf[k]);
+        for (int k = 0; k < K; ++k) {
+            at.load(w, 1.f, k, wf[k]);
+            at.load(b, 0.f, k, bf[k]);
+        }
     }
     const int64_t stride = (int64_t)gridDim.x * R;
     int64_t row = (int64_t)blockIdx.x * R + threadIdx.x / TPR;
     uint4 q[K];
     if (row < rows) at.load(x + row * cols, q);
     for (int turn = 0; row < rows; row += stride, turn ^= 1) {      // (a workgroup of one row leaves the loop as one: R == 1 with barriers)
+        int64_t again = 0;
+        if constexpr (!HOLD) asm volatile("" : "+s"(again));      // (an offset it cannot see through: else the compiler reads w, b once, and spills them)
         float f[K][V];
 #pragma unroll
         for (int k = 0; k < K; ++k) Chunk<T>::unpack(q[k], f[k]);
@@ -132,7 +184,7 @@ __global__ __launch_bounds__(block_threads(TPR)) void ln_fwd_kernel(const T* __r
         for (int k = 0; k < K; ++k)
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                const float d = FULL || e < at.valid(k) ? f[k][e] - m : 0.f;
+                const float d = at.whole(k) || e < at.valid(k) ? f[k][e] - m : 0.f;
                 ss = fmaf(d, d, ss);
             }
         ss = lanes_sum<(TPR < 64 ? TPR : 64)>(ss);
@@ -157,14 +209,19 @@ __global__ __launch_bounds__(block_threads(TPR)) void ln_fwd_kernel(const T* __r
         const float r = 1.f / sqrtf(fmaf(ss, inv, eps));
 #pragma unroll
         for (int k = 0; k < K; ++k) {
+            const int kw = HOLD ? k : 0;
+            if constexpr (!HOLD) {
+                at.load(w ? w + again : w, 1.f, k, wf[0]);
+                at.load(b ? b + again : b, 0.f, k, bf[0]);
+            }
             float y[V];
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                y[e] = fmaf((f[k][e] - m) * r, wf[k][e], bf[k][e]);
+                y[e] = fmaf((f[k][e] - m) * r, wf[kw][e], bf[kw][e]);
                 if (relu && y[e] < 0.f) y[e] = 0.f;          // (a NaN stays)
             }
             const int n = at.valid(k);
-            if (FULL || n > 0) store_chunk<T>(out + row * cols + at.col(k), n, y);
+            if (at.whole(k) || n > 0) store_chunk<T>(out + row * cols + at.col(k), n, y);
         }
         if (at.lane == 0) { mean[row] = m; rstd[row] = r; }
     }
@@ -174,7 +231,7 @@ __global__ __launch_bounds__(block_threads(TPR)) void ln_fwd_kernel(const T* __r
 // A thread has the same columns in every row it works on: its parts of dweight and dbias stay in registers until the last row.  Then the
 // R row groups of a workgroup are added up in LDS and one partial row [2][cols] a workgroup goes to scratch (or, with DIRECT, the only
 // workgroup writes the result).
-template <typename T, int TPR, int K, bool FULL>
+template <typename T, int TPR, int K, bool FULL, bool ACT>
 __global__ __launch_bounds__(block_threads(TPR)) void ln_bwd_kernel(const T* __restrict__ x, const float* __restrict__ w,
                                                                     const float* __restrict__ mean, const float* __restrict__ rstd,
                                                                     const T* __restrict__ dout, const T* __restrict__ act, T* __restrict__ dx,
@@ -184,26 +241,29 @@ __global__ __launch_bounds__(block_threads(TPR)) void ln_bwd_kernel(const T* __r
     const Cols<T, TPR, K, FULL> at(cols);
     const float inv = 1.f / (float)cols;
     __shared__ float2 part[2][WAVES > 1 ? WAVES : 1];
-    float wf[K][V], dw[K][V], db[K][V];
+    constexpr bool HOLD = holds_weights(TPR);
+    float wf[HOLD ? K : 1][V], dw[K][V], db[K][V];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-        load_vector<V>(w, at.col(k), at.valid(k), 1.f, wf[k]);
+        if constexpr (HOLD) at.load(w, 1.f, k, wf[k]);
 #pragma unroll
         for (int e = 0; e < V; ++e) dw[k][e] = db[k][e] = 0.f;
     }
     const int64_t stride = (int64_t)gridDim.x * R;
     int64_t row = (int64_t)blockIdx.x * R + threadIdx.x / TPR;
-    uint4 qx[K], qd[K], qa[K];
+    uint4 qx[K], qd[K], qa[ACT ? K : 1];
     float m_next = 0.f, r_next = 0.f;
     auto fetch = [&](int64_t i) {
         at.load(x + i * cols, qx);
         at.load(dout + i * cols, qd);
-        if (act) at.load(act + i * cols, qa);
+        if constexpr (ACT) at.load(act + i * cols, qa);
         m_next = mean[i];
         r_next = rstd[i];
     };
     if (row < rows) fetch(row);
     for (int turn = 0; row < rows; row += stride, turn ^= 1) {
+        int64_t again = 0;
+        if constexpr (!HOLD) asm volatile("" : "+s"(again));      // (see ln_fwd_kernel)
         float xh[K][V], g[K][V];
         const float m = m_next, r = r_next;
         float c1 = 0.f, c2 = 0.f;
@@ -211,7 +271,7 @@ __global__ __launch_bounds__(block_threads(TPR)) void ln_bwd_kernel(const T* __r
         for (int k = 0; k < K; ++k) {
             Chunk<T>::unpack(qx[k], xh[k]);
             Chunk<T>::unpack(qd[k], g[k]);
-            if (act) {
+            if constexpr (ACT) {
                 float a[V];
                 Chunk<T>::unpack(qa[k], a);
 #pragma unroll
@@ -220,16 +280,19 @@ __global__ __launch_bounds__(block_threads(TPR)) void ln_bwd_kernel(const T* __r
         }
         if (row + stride < rows) fetch(row + stride);
 #pragma unroll
-        for (int k = 0; k < K; ++k)
+        for (int k = 0; k < K; ++k) {
+            const int kw = HOLD ? k : 0;
+            if constexpr (!HOLD) at.load(w ? w + again : w, 1.f, k, wf[0]);
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                xh[k][e] = FULL || e < at.valid(k) ? (xh[k][e] - m) * r : 0.f;
+                xh[k][e] = at.whole(k) || e < at.valid(k) ? (xh[k][e] - m) * r : 0.f;
                 db[k][e] += g[k][e];
                 dw[k][e] = fmaf(g[k][e], xh[k][e], dw[k][e]);
-                g[k][e] *= wf[k][e];
+                g[k][e] *= wf[kw][e];
                 c1 += g[k][e];
                 c2 = fmaf(g[k][e], xh[k][e], c2);
             }
+        }
         c1 = lanes_sum<(TPR < 64 ? TPR : 64)>(c1);
         c2 = lanes_sum<(TPR < 64 ? TPR : 64)>(c2);
         if constexpr (WAVES > 1) {
@@ -247,7 +310,7 @@ __global__ __launch_bounds__(block_threads(TPR)) void ln_bwd_kernel(const T* __r
 #pragma unroll
             for (int e = 0; e < V; ++e) y[e] = r * (g[k][e] - c1 - xh[k][e] * c2);
             const int n = at.valid(k);
-            if (FULL || n > 0) store_chunk<T>(dx + row * cols + at.col(k), n, y);
+            if (at.whole(k) || n > 0) store_chunk<T>(dx + row * cols + at.col(k), n, y);
         }
     }
     if (!dw_out) return;
@@ -279,7 +342,7 @@ __global__ __launch_bounds__(block_threads(TPR)) void ln_bwd_kernel(const T* __r
             for (int k = 0; k < K; ++k)
 #pragma unroll
                 for (int e = 0; e < V; ++e)
-                    if (FULL || e < at.valid(k)) {
+                    if (at.whole(k) || e < at.valid(k)) {
                         const int c = at.col(k) + e;
                         to[c] = add ? to[c] + v[k][e] : v[k][e];
                     }
@@ -337,7 +400,7 @@ __global__ __launch_bounds__(1024) void ln_fwd_long_kernel(const T* __restrict__
         const T* xr = x + row * cols;
         float s = 0.f, f[V];
         for (int64_t c = threadIdx.x * V; c < cols; c += 1024 * V) {
-            Chunk<T>::unpack(load_chunk<T>(xr + c, cols - c < V ? (int)(cols - c) : V), f);
+            Chunk<T>::unpack(load_chunk<T, false>(xr, c, (int64_t)cols), f);
 #pragma unroll
             for (int e = 0; e < V; ++e) s += f[e];
         }
@@ -345,7 +408,7 @@ __global__ __launch_bounds__(1024) void ln_fwd_long_kernel(const T* __restrict__
         s = 0.f;
         for (int64_t c = threadIdx.x * V; c < cols; c += 1024 * V) {
             const int n = cols - c < V ? (int)(cols - c) : V;
-            Chunk<T>::unpack(load_chunk<T>(xr + c, n), f);
+            Chunk<T>::unpack(load_chunk<T, false>(xr, c, (int64_t)cols), f);
 #pragma unroll
             for (int e = 0; e < V; ++e) {
                 const float d = e < n ? f[e] - m : 0.f;
@@ -356,9 +419,9 @@ __global__ __launch_bounds__(1024) void ln_fwd_long_kernel(const T* __restrict__
         for (int64_t c = threadIdx.x * V; c < cols; c += 1024 * V) {
             const int n = cols - c < V ? (int)(cols - c) : V;
             float wf[V], bf[V];
-            Chunk<T>::unpack(load_chunk<T>(xr + c, n), f);
-            load_vector<V>(w, c, n, 1.f, wf);
-            load_vector<V>(b, c, n, 0.f, bf);
+            Chunk<T>::unpack(load_chunk<T, false>(xr, c, (int64_t)cols), f);
+            load_vector<V, false>(w, c, (int64_t)cols, 1.f, wf);
+            load_vector<V, false>(b, c, (int64_t)cols, 0.f, bf);
 #pragma unroll
             for (int e = 0; e < V; ++e) {
                 f[e] = fmaf((f[e] - m) * r, wf[e], bf[e]);
@@ -372,19 +435,19 @@ __global__ __launch_bounds__(1024) void ln_fwd_long_kernel(const T* __restrict__
 
 // d (masked) and xhat of one chunk
 template <typename T>
-__device__ __forceinline__ void grad_chunk(const T* __restrict__ x, const T* __restrict__ dout, const T* __restrict__ act, int64_t i, int n, float m,
-                                           float r, float* d, float* xh) {
+__device__ __forceinline__ void grad_chunk(const T* __restrict__ x, const T* __restrict__ dout, const T* __restrict__ act, int64_t row, int64_t c,
+                                           int cols, float m, float r, float* d, float* xh) {
     constexpr int V = Elem<T>::CH;
-    Chunk<T>::unpack(load_chunk<T>(x + i, n), xh);
-    Chunk<T>::unpack(load_chunk<T>(dout + i, n), d);
+    Chunk<T>::unpack(load_chunk<T, false>(x + row * cols, c, (int64_t)cols), xh);
+    Chunk<T>::unpack(load_chunk<T, false>(dout + row * cols, c, (int64_t)cols), d);
     if (act) {
         float a[V];
-        Chunk<T>::unpack(load_chunk<T>(act + i, n), a);
+        Chunk<T>::unpack(load_chunk<T, false>(act + row * cols, c, (int64_t)cols), a);
 #pragma unroll
         for (int e = 0; e < V; ++e) d[e] = a[e] > 0.f ? d[e] : 0.f;
     }
 #pragma unroll
-    for (int e = 0; e < V; ++e) xh[e] = e < n ? (xh[e] - m) * r : 0.f;
+    for (int e = 0; e < V; ++e) xh[e] = c + e < cols ? (xh[e] - m) * r : 0.f;
 }
 
 template <typename T>
@@ -398,8 +461,8 @@ __global__ __launch_bounds__(1024) void ln_bwd_long_dx_kernel(const T* __restric
         float c1 = 0.f, c2 = 0.f, d[V], xh[V], wf[V];
         for (int64_t c = threadIdx.x * V; c < cols; c += 1024 * V) {
             const int n = cols - c < V ? (int)(cols - c) : V;
-            grad_chunk<T>(x, dout, act, row * cols + c, n, m, r, d, xh);
-            load_vector<V>(w, c, n, 1.f, wf);
+            grad_chunk<T>(x, dout, act, row, c, cols, m, r, d, xh);
+            load_vector<V, false>(w, c, (int64_t)cols, 1.f, wf);
 #pragma unroll
             for (int e = 0; e < V; ++e) {
                 const float g = d[e] * wf[e];
@@ -411,8 +474,8 @@ __global__ __launch_bounds__(1024) void ln_bwd_long_dx_kernel(const T* __restric
         c2 = block_sum<16>(c2, red) / (float)cols;
         for (int64_t c = threadIdx.x * V; c < cols; c += 1024 * V) {
             const int n = cols - c < V ? (int)(cols - c) : V;
-            grad_chunk<T>(x, dout, act, row * cols + c, n, m, r, d, xh);
-            load_vector<V>(w, c, n, 1.f, wf);
+            grad_chunk<T>(x, dout, act, row, c, cols, m, r, d, xh);
+            load_vector<V, false>(w, c, (int64_t)cols, 1.f, wf);
 #pragma unroll
             for (int e = 0; e < V; ++e) d[e] = r * (d[e] * wf[e] - c1 - xh[e] * c2);
             store_chunk<T>(dx + row * cols + c, n, d);
@@ -434,7 +497,7 @@ __global__ __launch_bounds__(256) void ln_bwd_long_dw_kernel(const T* __restrict
     for (int e = 0; e < V; ++e) dw[e] = db[e] = 0.f;
 #pragma unroll 4
     for (int64_t row = blockIdx.y; row < rows; row += gridDim.y) {
-        grad_chunk<T>(x, dout, act, row * cols + c, n, mean[row], rstd[row], d, xh);
+        grad_chunk<T>(x, dout, act, row, c, cols, mean[row], rstd[row], d, xh);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
             db[e] += d[e];
@@ -514,12 +577,16 @@ struct BwdArgs {
 };
 
 template <typename T, int TPR, int K> void launch_bwd(const BwdArgs& a, hipStream_t st) {
-    if (a.cols == TPR * K * Elem<T>::CH)
-        hipLaunchKernelGGL((ln_bwd_kernel<T, TPR, K, true>), dim3(a.blocks), dim3(block_threads(TPR)), 0, st, (const T*)a.x, a.w, a.mean, a.rstd,
-                           (const T*)a.dout, (const T*)a.act, (T*)a.dx, a.dw, a.db, a.accumulate, a.partial, a.rows, a.cols);
-    else
-        hipLaunchKernelGGL((ln_bwd_kernel<T, TPR, K, false>), dim3(a.blocks), dim3(block_threads(TPR)), 0, st, (const T*)a.x, a.w, a.mean, a.rstd,
-                           (const T*)a.dout, (const T*)a.act, (T*)a.dx, a.dw, a.db, a.accumulate, a.partial, a.rows, a.cols);
+    const bool full = a.cols == TPR * K * Elem<T>::CH;
+#define LN_LAUNCH(FULL, ACT)                                                                                                              \
+    if (full == FULL && (a.act != nullptr) == ACT)                                                                                        \
+        hipLaunchKernelGGL((ln_bwd_kernel<T, TPR, K, FULL, ACT>), dim3(a.blocks), dim3(block_threads(TPR)), 0, st, (const T*)a.x, a.w, a.mean, \
+                           a.rstd, (const T*)a.dout, (const T*)a.act, (T*)a.dx, a.dw, a.db, a.accumulate, a.partial, a.rows, a.cols)
+    LN_LAUNCH(true, false);
+    LN_LAUNCH(true, true);
+    LN_LAUNCH(false, false);
+    LN_LAUNCH(false, true);
+#undef LN_LAUNCH
 }
 
 template <typename T> void run_bwd(const Split& s, const BwdArgs& a, hipStream_t st) {
