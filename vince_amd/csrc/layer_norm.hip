@@ -7,84 +7,80 @@
 // past what a workgroup's registers hold are read again for every pass (the *_long kernels).
 #include "common.h"
 
+// Where a row's end cuts a 16-byte chunk, two threads compute the columns that its chunk shares with the one before it, and both write
+// them: the same bits, so every multiply-add is written out (fmaf) and the compiler makes none by itself.
+#pragma clang fp contract(off)
+
 namespace {
 
-// ---- 16-byte chunks of a row at any element-aligned address ---------------------------------------------------------------------
+// ---- 16-byte chunks at any element-aligned address (the hardware takes any; the type tells the compiler so) --------------------------
 typedef __attribute__((ext_vector_type(4), aligned(2))) uint32_t u32x4_any_t;
-
 template <typename T> __device__ __forceinline__ uint4 load16(const T* __restrict__ p) {
     const u32x4_any_t v = *(const u32x4_any_t*)p;
     return make_uint4(v[0], v[1], v[2], v[3]);
 }
-// The chunk at column `col` of a row, zeros behind the row's end.  One load whatever the chunk holds: a chunk that the row's end cuts
-// is read as the row's last 16 bytes and shifted down (element by element it would be seven loads, or seven round trips).
-template <typename T, bool FULL, typename I> __device__ __forceinline__ uint4 load_chunk(const T* __restrict__ row, I col, I cols) {
-    constexpr int V = Elem<T>::CH, BITS = 8 * sizeof(T);
-    if constexpr (FULL) return load16<T>(row + col);
-    if (cols < V) {                                       // (a row of less than 16 bytes; uniform)
-        uint32_t u[4] = {0u, 0u, 0u, 0u};
-        if (col == 0)
-#pragma unroll
-            for (int e = 0; e < V - 1; ++e) {
-                const T one = row[e < cols ? e : 0];
-                uint32_t bits;
-                if constexpr (sizeof(T) == 4) bits = __float_as_uint(one);
-                else bits = one;
-                if (e < cols) u[e * sizeof(T) / 4] |= bits << (e * BITS % 32);
-            }
-        return make_uint4(u[0], u[1], u[2], u[3]);
-    }
-    const I last = cols - V, from = col < last ? col : last;
-    uint4 q = load16<T>(row + from);
-    if (col > last) {
-        const int shift = (int)(col - last < V ? col - last : V) * BITS;       // 128: nothing of the chunk is in the row
-        unsigned __int128 v = ((unsigned __int128)(((uint64_t)q.w << 32) | q.z) << 64) | (((uint64_t)q.y << 32) | q.x);
-        v = shift >= 128 ? 0 : v >> shift;
-        q = make_uint4((uint32_t)v, (uint32_t)(v >> 32), (uint32_t)(v >> 64), (uint32_t)(v >> 96));
-    }
-    return q;
-}
-// n elements of a chunk to p: whole, or the 4 / 2 / 1 elements that n is made of
-template <typename T> __device__ __forceinline__ void store_chunk(T* __restrict__ p, int n, const float* f) {
-    typedef __attribute__((ext_vector_type(2), aligned(2))) uint32_t u32x2_any_t;
-    typedef __attribute__((aligned(2))) uint32_t u32_any_t;
-    constexpr int V = Elem<T>::CH;
+template <typename T> __device__ __forceinline__ void store16(T* __restrict__ p, const float* f) {
     const uint4 q = Chunk<T>::pack(f);
-    if (n >= V) {
-        const u32x4_any_t v = {q.x, q.y, q.z, q.w};
-        *(u32x4_any_t*)p = v;
-        return;
+    const u32x4_any_t v = {q.x, q.y, q.z, q.w};
+    *(u32x4_any_t*)p = v;
+}
+// the first n elements of a chunk, one by one (rows of less than 16 bytes)
+template <typename T> __device__ __forceinline__ uint4 load_few(const T* __restrict__ p, int n) {
+    uint32_t u[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int e = 0; e < Elem<T>::CH - 1; ++e) {
+        const T one = p[e < n ? e : 0];
+        uint32_t bits;
+        if constexpr (sizeof(T) == 4) bits = __float_as_uint(one);
+        else bits = one;
+        if (e < n) u[e * sizeof(T) / 4] |= bits << (8 * sizeof(T) * e % 32);
     }
-    uint32_t a = q.x, b = q.y, c = q.z;
-    if (n & (V / 2)) {
-        const u32x2_any_t v = {a, b};
-        *(u32x2_any_t*)p = v;
-        p += V / 2;
-        a = c;
-        b = q.w;
+    return make_uint4(u[0], u[1], u[2], u[3]);
+}
+template <typename T> __device__ __forceinline__ void store_few(T* __restrict__ p, int n, const float* f) {
+#pragma unroll
+    for (int e = 0; e < Elem<T>::CH - 1; ++e)
+        if (e < n) {
+            if constexpr (sizeof(T) == 4) p[e] = f[e];
+            else p[e] = f32_to_bf16(f[e]);
+        }
+}
+
+// The chunk that starts at column `col` of a row of `cols`.  One that the row's end cuts is taken as the row's last 16 bytes: one load
+// and one store whatever it holds, nothing to shift; its first elements are the chunk's before it, and stay out of the sums (own()).
+// A chunk behind the row's end reads the row's last 16 bytes too, and owns nothing.  SHORT: the row may have less than 16 bytes.
+template <typename T, typename I, bool SHORT> struct Piece {
+    static constexpr int V = Elem<T>::CH;
+    I from;
+    int first, n, cols;          // its own elements are first .. first + n - 1
+    __device__ __forceinline__ Piece(I col, I cols_) {
+        const bool small = SHORT && cols_ < V;
+        cols = small ? (int)cols_ : V;
+        const I last = small ? 0 : cols_ - V;
+        from = col < last ? col : last;
+        first = (int)(col - from < V ? col - from : V);
+        n = small ? (col == 0 ? (int)cols_ : 0) : V - first;
     }
-    if constexpr (sizeof(T) == 2) {
-        if (n & 2) {
-            *(u32_any_t*)p = a;
-            p += 2;
-            a = b;
+    __device__ __forceinline__ bool own(int e) const { return SHORT ? (unsigned)(e - first) < (unsigned)n : e >= first; }
+    __device__ __forceinline__ uint4 load(const T* __restrict__ row) const {
+        if (SHORT && cols < V) return load_few<T>(row, cols);
+        return load16<T>(row + from);
+    }
+    __device__ __forceinline__ void load_vector(const float* __restrict__ p, float none, float* f) const {
+        if (!p || (SHORT && cols < V)) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) f[e] = SHORT && p && e < cols ? p[e] : none;
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; e += 4) Chunk<float>::unpack(load16<float>(p + from + e), f + e);
         }
     }
-    if (n & 1) {
-        if constexpr (sizeof(T) == 4) *p = __uint_as_float(a);
-        else *p = (bf16_t)a;
+    __device__ __forceinline__ void store(T* __restrict__ row, const float* f) const {
+        if (n == 0) return;
+        if (SHORT && cols < V) store_few<T>(row, cols, f);
+        else store16<T>(row + from, f);
     }
-}
-// the same columns of an fp32 vector (NULL: `none` everywhere)
-template <int V, bool FULL, typename I> __device__ __forceinline__ void load_vector(const float* __restrict__ p, I col, I cols, float none, float* f) {
-    if (!p) {
-#pragma unroll
-        for (int e = 0; e < V; ++e) f[e] = none;
-        return;
-    }
-#pragma unroll
-    for (int e = 0; e < V; e += 4) Chunk<float>::unpack(load_chunk<float, FULL>(p, (I)(col + e), cols), f + e);
-}
+};
 
 // ---- sums over groups of lanes, every lane with the same bits ---------------------------------------------------------------------
 template <int CTRL> __device__ __forceinline__ float dpp(float v) {
@@ -106,31 +102,60 @@ template <int N> __device__ __forceinline__ float lanes_sum(float v) {   // N = 
     return v;
 }
 
-constexpr int block_threads(int tpr) { return tpr > 256 ? tpr : 256; }
-// Whether a thread keeps its columns' weight (and bias) in registers from row to row.  At 1024 threads, with 128 registers each, there is
-// no room: they are read again for every row, from the caches.
-constexpr bool holds_weights(int tpr) { return tpr < 1024; }
+// the sum over the wavefront's lanes l, l + 8, l + 16, ... in each of them
+template <int N> __device__ __forceinline__ float strided_sum(float v) {
+    static_assert(N == 8, "lanes 8 apart");
+    v += dpp<0x128>(v);                            // row_ror:8
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
 
-// Where this thread's K chunks of a row are.  FULL: cols == TPR * K * V, every chunk whole.  Else the first K / 2 are (ln_split takes K > 1
-// for rows of more than TPR * K / 2 chunks), the others may be cut by the row's end or lie behind it.
+constexpr int block_threads(int tpr) { return tpr > 64 ? tpr : 256; }
+constexpr int wave_lanes(int tpr) { return tpr < 64 ? tpr : 64; }
+// Whether a thread keeps its columns' weight (and bias) in registers from row to row.  At 1024 threads, with 128 registers each, there is
+// room for 8 values only: else they are read again for every row, from the caches.
+constexpr bool holds_weights(int tpr, int values) { return tpr < 1024 || values <= 8; }
+
+// s / n from inv = 1 / n, with one step of correction: exact where the quotient is a float, so that a row of one value has that mean and
+// the bias as its output; a third of the instructions of a division, which every wavefront would make for every row
+__device__ __forceinline__ float divide(float s, float n, float inv) {
+    const float q = s * inv, better = fmaf(fmaf(-q, n, s), inv, q);
+    return better == better ? better : q;          // (an infinite sum: the correction is NaN)
+}
+
+// This thread's K chunks of a row.  FULL: cols == TPR * K * V, every chunk whole.  Else the first K / 2 are (ln_split takes K > 1 for rows
+// of more than TPR * K / 2 chunks).
 template <typename T, int TPR, int K, bool FULL> struct Cols {
     static constexpr int V = Elem<T>::CH;
     int lane, cols;
     __device__ __forceinline__ Cols(int cols_) : lane((int)threadIdx.x % TPR), cols(cols_) {}
-    __device__ __forceinline__ int col(int k) const { return (k * TPR + lane) * V; }
     static constexpr bool whole(int k) { return FULL || k < K / 2; }
-    __device__ __forceinline__ int valid(int k) const {   // elements of chunk k that are in the row
-        if (whole(k)) return V;
-        const int n = cols - col(k);
-        return n < 0 ? 0 : n > V ? V : n;
-    }
+    __device__ __forceinline__ int col(int k) const { return (k * TPR + lane) * V; }
+    typedef Piece<T, int, TPR == 2> piece_t;             // (only rows of one or two chunks can have less than 16 bytes)
+    __device__ __forceinline__ piece_t piece(int k) const { return piece_t(col(k), cols); }
+    __device__ __forceinline__ bool own(int k, int e) const { return whole(k) || piece(k).own(e); }
+    __device__ __forceinline__ int own(int k) const { return whole(k) ? V : piece(k).n; }
+    __device__ __forceinline__ int first_col(int k) const { return whole(k) ? col(k) : piece(k).from; }
     __device__ __forceinline__ void load(const T* __restrict__ row, uint4 (&q)[K]) const {
 #pragma unroll
-        for (int k = 0; k < K; ++k) q[k] = whole(k) ? load_chunk<T, true>(row, col(k), cols) : load_chunk<T, false>(row, col(k), cols);
+        for (int k = 0; k < K; ++k) q[k] = whole(k) ? load16<T>(row + col(k)) : piece(k).load(row);
     }
     __device__ __forceinline__ void load(const float* __restrict__ p, float none, int k, float (&f)[V]) const {   // of a vector of the row's length
-        if (whole(k)) load_vector<V, true>(p, col(k), cols, none, f);
-        else load_vector<V, false>(p, col(k), cols, none, f);
+        if (whole(k) && p) {
+#pragma unroll
+            for (int e = 0; e < V; e += 4) Chunk<float>::unpack(load16<float>(p + col(k) + e), f + e);
+        } else if (whole(k)) {
+#pragma unroll
+            for (int e = 0; e < V; ++e) f[e] = none;
+        } else {
+            piece(k).load_vector(p, none, f);
+        }
+    }
+    __device__ __forceinline__ void store(T* __restrict__ row, int k, const float (&f)[V]) const {
+        if (whole(k)) store16<T>(row + col(k), f);
+        else piece(k).store(row, f);
     }
 };
 
@@ -138,21 +163,24 @@ template <typename T, int TPR, int K, bool FULL>
 __global__ __launch_bounds__(block_threads(TPR)) void ln_fwd_kernel(const T* __restrict__ x, const float* __restrict__ w,
                                                                     const float* __restrict__ b, T* __restrict__ out, float* __restrict__ mean,
                                                                     float* __restrict__ rstd, int64_t rows, int cols, float eps, int relu) {
-    constexpr int V = Elem<T>::CH, R = block_threads(TPR) / TPR, WAVES = TPR / 64;
+    constexpr int V = Elem<T>::CH, R = block_threads(TPR) / TPR, WAVES = TPR / 64, LANES = wave_lanes(TPR);
+    constexpr bool HOLD = holds_weights(TPR, K * V);
     const Cols<T, TPR, K, FULL> at(cols);
     const float inv = 1.f / (float)cols;
     __shared__ float2 part[2][WAVES > 1 ? WAVES : 1];    // mean and squares of each wavefront's columns, two rows' worth
-    float count = 0.f;                                    // elements of a row that this wavefront's (or group's) lanes hold
-#pragma unroll
-    for (int k = 0; k < K; ++k) count += (float)at.valid(k);
-    count = lanes_sum<(TPR < 64 ? TPR : 64)>(count);
-    if (FULL) count = (float)((TPR < 64 ? TPR : 64) * K * V);
     __shared__ float counts[WAVES > 1 ? WAVES : 1];
-    if constexpr (WAVES > 1) {
-        if ((threadIdx.x & 63) == 0) counts[threadIdx.x >> 6] = count;
-        __syncthreads();
+    float count = (float)(LANES * K * V);                 // elements of a row that this wavefront's (or group's) lanes own
+    if constexpr (!FULL) {
+        count = 0.f;
+#pragma unroll
+        for (int k = 0; k < K; ++k) count += (float)at.own(k);
+        count = lanes_sum<LANES>(count);
+        if constexpr (WAVES > 1) {
+            if ((threadIdx.x & 63) == 0) counts[threadIdx.x >> 6] = count;
+            __syncthreads();
+        }
     }
-    constexpr bool HOLD = holds_weights(TPR);
+    const float inv_count = count > 0.f ? 1.f / count : 0.f;
     float wf[HOLD ? K : 1][V], bf[HOLD ? K : 1][V];
     if constexpr (HOLD) {
 #pragma unroll
@@ -165,7 +193,7 @@ __global__ __launch_bounds__(block_threads(TPR)) void ln_fwd_kernel(const T* __r
     int64_t row = (int64_t)blockIdx.x * R + threadIdx.x / TPR;
     uint4 q[K];
     if (row < rows) at.load(x + row * cols, q);
-    for (int turn = 0; row < rows; row += stride, turn ^= 1) {      // (a workgroup of one row leaves the loop as one: R == 1 with barriers)
+    for (int turn = 0; row < rows; row += stride, turn ^= 1) {      // (a workgroup with barriers has one row at a time: it leaves as one)
         int64_t again = 0;
         if constexpr (!HOLD) asm volatile("" : "+s"(again));      // (an offset it cannot see through: else the compiler reads w, b once, and spills them)
         float f[K][V];
@@ -176,18 +204,17 @@ __global__ __launch_bounds__(block_threads(TPR)) void ln_fwd_kernel(const T* __r
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
-            for (int e = 0; e < V; ++e) s += f[k][e];
-        // means by division, not by a rounded reciprocal: a row of one value has exactly that mean, and its output is the bias
-        float m = lanes_sum<(TPR < 64 ? TPR : 64)>(s) / fmaxf(count, 1.f);
+            for (int e = 0; e < V; ++e) s += at.own(k, e) ? f[k][e] : 0.f;
+        float m = divide(lanes_sum<LANES>(s), count, inv_count);
         float ss = 0.f;
 #pragma unroll
         for (int k = 0; k < K; ++k)
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                const float d = at.whole(k) || e < at.valid(k) ? f[k][e] - m : 0.f;
+                const float d = at.own(k, e) ? f[k][e] - m : 0.f;
                 ss = fmaf(d, d, ss);
             }
-        ss = lanes_sum<(TPR < 64 ? TPR : 64)>(ss);
+        ss = lanes_sum<LANES>(ss);
         if constexpr (WAVES > 1) {       // the row's from the wavefronts': their squares about their own means, moved to the common one
             if ((threadIdx.x & 63) == 0) part[turn][threadIdx.x >> 6] = make_float2(m, ss);
             __syncthreads();             // (the other turn's slot is written only behind the next row's barrier: one barrier a row)
@@ -196,17 +223,17 @@ __global__ __launch_bounds__(block_threads(TPR)) void ln_fwd_kernel(const T* __r
 #pragma unroll
             for (int i = 0; i < WAVES; ++i) {
                 p[i] = part[turn][i];
-                m = fmaf(p[i].x, FULL ? (float)(64 * K * V) : counts[i], m);
+                m = fmaf(p[i].x, FULL ? count : counts[i], m);
             }
-            m /= (float)cols;
+            m = divide(m, (float)cols, inv);
             ss = 0.f;
 #pragma unroll
             for (int i = 0; i < WAVES; ++i) {
                 const float d = p[i].x - m;
-                ss += fmaf(d * d, FULL ? (float)(64 * K * V) : counts[i], p[i].y);
+                ss += fmaf(d * d, FULL ? count : counts[i], p[i].y);
             }
         }
-        const float r = 1.f / sqrtf(fmaf(ss, inv, eps));
+        const float r = rsqrtf(fmaf(ss, inv, eps));
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             const int kw = HOLD ? k : 0;
@@ -216,32 +243,77 @@ __global__ __launch_bounds__(block_threads(TPR)) void ln_fwd_kernel(const T* __r
             }
             float y[V];
 #pragma unroll
-            for (int e = 0; e < V; ++e) {
-                y[e] = fmaf((f[k][e] - m) * r, wf[kw][e], bf[kw][e]);
-                if (relu && y[e] < 0.f) y[e] = 0.f;          // (a NaN stays)
+            for (int e = 0; e < V; ++e) y[e] = fmaf((f[k][e] - m) * r, wf[kw][e], bf[kw][e]);
+            if (relu) {
+                asm volatile("");                            // (a branch: two instructions an element for those who want none)
+#pragma unroll
+                for (int e = 0; e < V; ++e) y[e] = y[e] < 0.f ? 0.f : y[e];          // (a NaN stays)
             }
-            const int n = at.valid(k);
-            if (at.whole(k) || n > 0) store_chunk<T>(out + row * cols + at.col(k), n, y);
+            at.store(out + row * cols, k, y);
         }
         if (at.lane == 0) { mean[row] = m; rstd[row] = r; }
     }
 }
 
-// ---- backward: dx, and this workgroup's sums for dweight and dbias ------------------------------------------------------------------
-// A thread has the same columns in every row it works on: its parts of dweight and dbias stay in registers until the last row.  Then the
-// R row groups of a workgroup are added up in LDS and one partial row [2][cols] a workgroup goes to scratch (or, with DIRECT, the only
-// workgroup writes the result).
+// ---- backward ---------------------------------------------------------------------------------------------------------------------------
+// A row's chunks of x, dout and act in registers.
+template <typename T, int K, bool ACT> struct RowData {
+    static constexpr int V = Elem<T>::CH;
+    uint4 x[K], d[K], a[ACT ? K : 1];
+    float mean, rstd;
+    template <typename C>
+    __device__ __forceinline__ void load(const C& at, const T* __restrict__ xs, const T* __restrict__ dout, const T* __restrict__ act,
+                                         const float* __restrict__ ms, const float* __restrict__ rs, int64_t row, int cols) {
+        at.load(xs + row * cols, x);
+        at.load(dout + row * cols, d);
+        if constexpr (ACT) at.load(act + row * cols, a);
+        mean = ms[row];
+        rstd = rs[row];
+    }
+    __device__ __forceinline__ void unpack(float (&xv)[K][V], float (&g)[K][V]) const {      // x, and dout behind the ReLU
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            Chunk<T>::unpack(x[k], xv[k]);
+            Chunk<T>::unpack(d[k], g[k]);
+            if constexpr (ACT) {
+                float av[V];
+                Chunk<T>::unpack(a[k], av);
+#pragma unroll
+                for (int e = 0; e < V; ++e) g[k][e] = av[e] > 0.f ? g[k][e] : 0.f;
+            }
+        }
+    }
+};
+
+// the row's averages of g and g xhat from this thread's sums
+template <int TPR, int WAVES>
+__device__ __forceinline__ void row_averages(float& c1, float& c2, float2* part, float inv) {
+    c1 = lanes_sum<wave_lanes(TPR)>(c1);
+    c2 = lanes_sum<wave_lanes(TPR)>(c2);
+    if constexpr (WAVES > 1) {
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = make_float2(c1, c2);
+        __syncthreads();
+        c1 = c2 = 0.f;
+#pragma unroll
+        for (int i = 0; i < WAVES; ++i) { c1 += part[i].x; c2 += part[i].y; }
+    }
+    c1 *= inv;
+    c2 *= inv;
+}
+
+// dx, and this workgroup's sums for dweight and dbias.  A thread has the same columns in every row it works on: its parts of dweight and
+// dbias stay in registers until the last row.  Then the R row groups of a workgroup are added up in LDS and one partial row [2][cols] a
+// workgroup goes to scratch (partial == NULL: no weight, no sums).
 template <typename T, int TPR, int K, bool FULL, bool ACT>
 __global__ __launch_bounds__(block_threads(TPR)) void ln_bwd_kernel(const T* __restrict__ x, const float* __restrict__ w,
                                                                     const float* __restrict__ mean, const float* __restrict__ rstd,
                                                                     const T* __restrict__ dout, const T* __restrict__ act, T* __restrict__ dx,
-                                                                    float* __restrict__ dw_out, float* __restrict__ db_out, int accumulate,
                                                                     float* __restrict__ partial, int64_t rows, int cols) {
     constexpr int V = Elem<T>::CH, THREADS = block_threads(TPR), R = THREADS / TPR, WAVES = TPR / 64;
+    constexpr bool HOLD = holds_weights(TPR, K * V);
     const Cols<T, TPR, K, FULL> at(cols);
     const float inv = 1.f / (float)cols;
     __shared__ float2 part[2][WAVES > 1 ? WAVES : 1];
-    constexpr bool HOLD = holds_weights(TPR);
     float wf[HOLD ? K : 1][V], dw[K][V], db[K][V];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -251,101 +323,161 @@ __global__ __launch_bounds__(block_threads(TPR)) void ln_bwd_kernel(const T* __r
     }
     const int64_t stride = (int64_t)gridDim.x * R;
     int64_t row = (int64_t)blockIdx.x * R + threadIdx.x / TPR;
-    uint4 qx[K], qd[K], qa[ACT ? K : 1];
-    float m_next = 0.f, r_next = 0.f;
-    auto fetch = [&](int64_t i) {
-        at.load(x + i * cols, qx);
-        at.load(dout + i * cols, qd);
-        if constexpr (ACT) at.load(act + i * cols, qa);
-        m_next = mean[i];
-        r_next = rstd[i];
-    };
-    if (row < rows) fetch(row);
+    RowData<T, K, ACT> in;
+    if (row < rows) in.load(at, x, dout, act, mean, rstd, row, cols);
     for (int turn = 0; row < rows; row += stride, turn ^= 1) {
         int64_t again = 0;
         if constexpr (!HOLD) asm volatile("" : "+s"(again));      // (see ln_fwd_kernel)
         float xh[K][V], g[K][V];
-        const float m = m_next, r = r_next;
+        in.unpack(xh, g);
+        const float m = in.mean, r = in.rstd;
+        if (row + stride < rows) in.load(at, x, dout, act, mean, rstd, row + stride, cols);
         float c1 = 0.f, c2 = 0.f;
-#pragma unroll
-        for (int k = 0; k < K; ++k) {
-            Chunk<T>::unpack(qx[k], xh[k]);
-            Chunk<T>::unpack(qd[k], g[k]);
-            if constexpr (ACT) {
-                float a[V];
-                Chunk<T>::unpack(qa[k], a);
-#pragma unroll
-                for (int e = 0; e < V; ++e) g[k][e] = a[e] > 0.f ? g[k][e] : 0.f;
-            }
-        }
-        if (row + stride < rows) fetch(row + stride);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             const int kw = HOLD ? k : 0;
             if constexpr (!HOLD) at.load(w ? w + again : w, 1.f, k, wf[0]);
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                xh[k][e] = at.whole(k) || e < at.valid(k) ? (xh[k][e] - m) * r : 0.f;
-                db[k][e] += g[k][e];
-                dw[k][e] = fmaf(g[k][e], xh[k][e], dw[k][e]);
+                xh[k][e] = (xh[k][e] - m) * r;
+                const float d = at.own(k, e) ? g[k][e] : 0.f;
+                db[k][e] += d;
+                dw[k][e] = fmaf(d, xh[k][e], dw[k][e]);
                 g[k][e] *= wf[kw][e];
-                c1 += g[k][e];
-                c2 = fmaf(g[k][e], xh[k][e], c2);
+                const float go = at.own(k, e) ? g[k][e] : 0.f;
+                c1 += go;
+                c2 = fmaf(go, xh[k][e], c2);
             }
         }
-        c1 = lanes_sum<(TPR < 64 ? TPR : 64)>(c1);
-        c2 = lanes_sum<(TPR < 64 ? TPR : 64)>(c2);
-        if constexpr (WAVES > 1) {
-            if ((threadIdx.x & 63) == 0) part[turn][threadIdx.x >> 6] = make_float2(c1, c2);
-            __syncthreads();
-            c1 = c2 = 0.f;
-#pragma unroll
-            for (int i = 0; i < WAVES; ++i) { c1 += part[turn][i].x; c2 += part[turn][i].y; }
-        }
-        c1 *= inv;
-        c2 *= inv;
+        row_averages<TPR, WAVES>(c1, c2, part[turn], inv);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             float y[V];
 #pragma unroll
-            for (int e = 0; e < V; ++e) y[e] = r * (g[k][e] - c1 - xh[k][e] * c2);
-            const int n = at.valid(k);
-            if (at.whole(k) || n > 0) store_chunk<T>(dx + row * cols + at.col(k), n, y);
+            for (int e = 0; e < V; ++e) y[e] = r * fmaf(-xh[k][e], c2, g[k][e] - c1);
+            at.store(dx + row * cols, k, y);
         }
     }
-    if (!dw_out) return;
+    if (!partial) return;
     // one row group a workgroup: the registers are the workgroup's sums; several: added up in LDS in the order of the groups
-    __shared__ float red[R > 1 ? THREADS * K * V : 1];
+    __shared__ float red[R > 1 ? R * TPR * K * V : 1];
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
         float(&v)[K][V] = half == 0 ? dw : db;
+        float* to = partial + ((int64_t)blockIdx.x * 2 + half) * cols;
         if constexpr (R > 1) {
             __syncthreads();
 #pragma unroll
             for (int k = 0; k < K; ++k)
 #pragma unroll
-                for (int e = 0; e < V; ++e) red[(threadIdx.x / TPR * K + k) * (TPR * V) + at.lane * V + e] = v[k][e];
+                for (int e = 0; e < V; ++e)
+                    if (at.own(k, e)) red[threadIdx.x / TPR * (TPR * K * V) + at.first_col(k) + e] = v[k][e];
             __syncthreads();
-        }
-        float* final_out = half == 0 ? dw_out : db_out;
-        float* to = partial ? partial + ((int64_t)blockIdx.x * 2 + half) * cols : final_out;
-        const bool add = !partial && accumulate;
-        if constexpr (R > 1) {
-            for (int c = threadIdx.x; c < cols; c += THREADS) {       // (cols <= TPR * K * V)
+            for (int c = threadIdx.x; c < cols; c += THREADS) {
                 float s = 0.f;
 #pragma unroll 8
-                for (int i = 0; i < R; ++i) s += red[i * (K * TPR * V) + c];
-                to[c] = add ? to[c] + s : s;
+                for (int i = 0; i < R; ++i) s += red[i * (TPR * K * V) + c];
+                to[c] = s;
             }
         } else {
 #pragma unroll
             for (int k = 0; k < K; ++k)
 #pragma unroll
                 for (int e = 0; e < V; ++e)
-                    if (at.whole(k) || e < at.valid(k)) {
-                        const int c = at.col(k) + e;
-                        to[c] = add ? to[c] + v[k][e] : v[k][e];
-                    }
+                    if (at.own(k, e)) to[at.first_col(k) + e] = v[k][e];
+        }
+    }
+}
+
+// Few rows: one launch.  dweight and dbias need the given mean and rstd only, not what dx needs from a whole row, so workgroups of their
+// own sum 8 chunks of columns each over all rows, beside those that compute dx; x and dout are read twice (the second time from a
+// cache), nothing goes through scratch.
+template <typename T, int TPR, int K, bool ACT>
+__global__ __launch_bounds__(block_threads(TPR)) void ln_bwd_few_kernel(const T* __restrict__ x, const float* __restrict__ w,
+                                                                        const float* __restrict__ mean, const float* __restrict__ rstd,
+                                                                        const T* __restrict__ dout, const T* __restrict__ act,
+                                                                        T* __restrict__ dx, float* __restrict__ dw_out,
+                                                                        float* __restrict__ db_out, int accumulate, int rows, int cols,
+                                                                        int dx_blocks) {
+    constexpr int V = Elem<T>::CH, THREADS = block_threads(TPR), R = THREADS / TPR, WAVES = TPR / 64;
+    if ((int)blockIdx.x < dx_blocks) {
+        const Cols<T, TPR, K, false> at(cols);
+        __shared__ float2 part[WAVES > 1 ? WAVES : 1];
+        const int row = (int)blockIdx.x * R + (int)threadIdx.x / TPR;
+        if (row >= rows) return;                            // (with barriers a workgroup has one row: it leaves as one)
+        RowData<T, K, ACT> in;
+        in.load(at, x, dout, act, mean, rstd, row, cols);
+        float xh[K][V], g[K][V], c1 = 0.f, c2 = 0.f;
+        in.unpack(xh, g);
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            float wf[V];
+            at.load(w, 1.f, k, wf);
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                xh[k][e] = (xh[k][e] - in.mean) * in.rstd;
+                g[k][e] *= wf[e];
+                const float go = at.own(k, e) ? g[k][e] : 0.f;
+                c1 += go;
+                c2 = fmaf(go, xh[k][e], c2);
+            }
+        }
+        row_averages<TPR, WAVES>(c1, c2, part, 1.f / (float)cols);
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            float y[V];
+#pragma unroll
+            for (int e = 0; e < V; ++e) y[e] = in.rstd * fmaf(-xh[k][e], c2, g[k][e] - c1);
+            at.store(dx + (int64_t)row * cols, k, y);
+        }
+        return;
+    }
+    constexpr int LANES = 8, ROWS = THREADS / LANES;
+    __shared__ float red[2][THREADS / 64][LANES * V];
+    const int lane = (int)threadIdx.x % LANES;
+    const Piece<T, int, TPR == 2> piece((((int)blockIdx.x - dx_blocks) * LANES + lane) * V, cols);
+    float dw[V], db[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) dw[e] = db[e] = 0.f;
+#pragma unroll 4
+    for (int row = (int)threadIdx.x / LANES; row < rows; row += ROWS) {
+        const int64_t i = (int64_t)row * cols;
+        float xv[V], d[V];
+        Chunk<T>::unpack(piece.load(x + i), xv);
+        Chunk<T>::unpack(piece.load(dout + i), d);
+        if constexpr (ACT) {
+            float a[V];
+            Chunk<T>::unpack(piece.load(act + i), a);
+#pragma unroll
+            for (int e = 0; e < V; ++e) d[e] = a[e] > 0.f ? d[e] : 0.f;
+        }
+        const float m = mean[row], r = rstd[row];
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            db[e] += d[e];
+            dw[e] = fmaf(d[e], (xv[e] - m) * r, dw[e]);
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        const float sw = strided_sum<LANES>(dw[e]), sb = strided_sum<LANES>(db[e]);
+        if ((threadIdx.x & 63) < LANES) {
+            red[0][threadIdx.x >> 6][lane * V + e] = sw;
+            red[1][threadIdx.x >> 6][lane * V + e] = sb;
+        }
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < LANES) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            float sw = 0.f, sb = 0.f;
+#pragma unroll
+            for (int i = 0; i < THREADS / 64; ++i) { sw += red[0][i][lane * V + e]; sb += red[1][i][lane * V + e]; }
+            if (piece.own(e)) {
+                const int c = piece.from + e;
+                dw_out[c] = accumulate ? dw_out[c] + sw : sw;
+                db_out[c] = accumulate ? db_out[c] + sb : sb;
+            }
         }
     }
 }
@@ -379,14 +511,14 @@ __global__ __launch_bounds__(1024) void ln_bwd_join_kernel(const float* __restri
 }
 
 // ---- rows longer than a workgroup's registers -----------------------------------------------------------------------------------------
-template <int WAVES> __device__ __forceinline__ float block_sum(float v, float* red) {
+__device__ __forceinline__ float sum_of_1024(float v, float* red) {
     v = lanes_sum<64>(v);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
     float s = 0.f;
 #pragma unroll
-    for (int i = 0; i < WAVES; ++i) s += red[i];
+    for (int i = 0; i < 16; ++i) s += red[i];
     return s;
 }
 
@@ -399,55 +531,59 @@ __global__ __launch_bounds__(1024) void ln_fwd_long_kernel(const T* __restrict__
     for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
         const T* xr = x + row * cols;
         float s = 0.f, f[V];
+#pragma unroll 4
         for (int64_t c = threadIdx.x * V; c < cols; c += 1024 * V) {
-            Chunk<T>::unpack(load_chunk<T, false>(xr, c, (int64_t)cols), f);
+            const Piece<T, int64_t, false> piece(c, cols);
+            Chunk<T>::unpack(piece.load(xr), f);
 #pragma unroll
-            for (int e = 0; e < V; ++e) s += f[e];
+            for (int e = 0; e < V; ++e) s += piece.own(e) ? f[e] : 0.f;
         }
-        const float m = block_sum<16>(s, red) / (float)cols;
+        const float m = sum_of_1024(s, red) / (float)cols;
         s = 0.f;
+#pragma unroll 4
         for (int64_t c = threadIdx.x * V; c < cols; c += 1024 * V) {
-            const int n = cols - c < V ? (int)(cols - c) : V;
-            Chunk<T>::unpack(load_chunk<T, false>(xr, c, (int64_t)cols), f);
+            const Piece<T, int64_t, false> piece(c, cols);
+            Chunk<T>::unpack(piece.load(xr), f);
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                const float d = e < n ? f[e] - m : 0.f;
+                const float d = piece.own(e) ? f[e] - m : 0.f;
                 s = fmaf(d, d, s);
             }
         }
-        const float r = 1.f / sqrtf(block_sum<16>(s, red) / (float)cols + eps);
+        const float r = 1.f / sqrtf(sum_of_1024(s, red) / (float)cols + eps);
+#pragma unroll 2
         for (int64_t c = threadIdx.x * V; c < cols; c += 1024 * V) {
-            const int n = cols - c < V ? (int)(cols - c) : V;
+            const Piece<T, int64_t, false> piece(c, cols);
             float wf[V], bf[V];
-            Chunk<T>::unpack(load_chunk<T, false>(xr, c, (int64_t)cols), f);
-            load_vector<V, false>(w, c, (int64_t)cols, 1.f, wf);
-            load_vector<V, false>(b, c, (int64_t)cols, 0.f, bf);
+            Chunk<T>::unpack(piece.load(xr), f);
+            piece.load_vector(w, 1.f, wf);
+            piece.load_vector(b, 0.f, bf);
 #pragma unroll
             for (int e = 0; e < V; ++e) {
                 f[e] = fmaf((f[e] - m) * r, wf[e], bf[e]);
                 if (relu && f[e] < 0.f) f[e] = 0.f;
             }
-            store_chunk<T>(out + row * cols + c, n, f);
+            piece.store(out + row * cols, f);
         }
         if (threadIdx.x == 0) { mean[row] = m; rstd[row] = r; }
     }
 }
 
-// d (masked) and xhat of one chunk
+// d (dout behind the ReLU) and xhat of one chunk
 template <typename T>
-__device__ __forceinline__ void grad_chunk(const T* __restrict__ x, const T* __restrict__ dout, const T* __restrict__ act, int64_t row, int64_t c,
-                                           int cols, float m, float r, float* d, float* xh) {
+__device__ __forceinline__ void grad_piece(const Piece<T, int64_t, false>& piece, const T* __restrict__ x, const T* __restrict__ dout,
+                                           const T* __restrict__ act, int64_t at, float m, float r, float* d, float* xh) {
     constexpr int V = Elem<T>::CH;
-    Chunk<T>::unpack(load_chunk<T, false>(x + row * cols, c, (int64_t)cols), xh);
-    Chunk<T>::unpack(load_chunk<T, false>(dout + row * cols, c, (int64_t)cols), d);
+    Chunk<T>::unpack(piece.load(x + at), xh);
+    Chunk<T>::unpack(piece.load(dout + at), d);
     if (act) {
         float a[V];
-        Chunk<T>::unpack(load_chunk<T, false>(act + row * cols, c, (int64_t)cols), a);
+        Chunk<T>::unpack(piece.load(act + at), a);
 #pragma unroll
         for (int e = 0; e < V; ++e) d[e] = a[e] > 0.f ? d[e] : 0.f;
     }
 #pragma unroll
-    for (int e = 0; e < V; ++e) xh[e] = c + e < cols ? (xh[e] - m) * r : 0.f;
+    for (int e = 0; e < V; ++e) xh[e] = (xh[e] - m) * r;
 }
 
 template <typename T>
@@ -459,26 +595,28 @@ __global__ __launch_bounds__(1024) void ln_bwd_long_dx_kernel(const T* __restric
     for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
         const float m = mean[row], r = rstd[row];
         float c1 = 0.f, c2 = 0.f, d[V], xh[V], wf[V];
+#pragma unroll 2
         for (int64_t c = threadIdx.x * V; c < cols; c += 1024 * V) {
-            const int n = cols - c < V ? (int)(cols - c) : V;
-            grad_chunk<T>(x, dout, act, row, c, cols, m, r, d, xh);
-            load_vector<V, false>(w, c, (int64_t)cols, 1.f, wf);
+            const Piece<T, int64_t, false> piece(c, cols);
+            grad_piece<T>(piece, x, dout, act, row * cols, m, r, d, xh);
+            piece.load_vector(w, 1.f, wf);
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                const float g = d[e] * wf[e];
+                const float g = piece.own(e) ? d[e] * wf[e] : 0.f;
                 c1 += g;
                 c2 = fmaf(g, xh[e], c2);
             }
         }
-        c1 = block_sum<16>(c1, red) / (float)cols;
-        c2 = block_sum<16>(c2, red) / (float)cols;
+        c1 = sum_of_1024(c1, red) / (float)cols;
+        c2 = sum_of_1024(c2, red) / (float)cols;
+#pragma unroll 2
         for (int64_t c = threadIdx.x * V; c < cols; c += 1024 * V) {
-            const int n = cols - c < V ? (int)(cols - c) : V;
-            grad_chunk<T>(x, dout, act, row, c, cols, m, r, d, xh);
-            load_vector<V, false>(w, c, (int64_t)cols, 1.f, wf);
+            const Piece<T, int64_t, false> piece(c, cols);
+            grad_piece<T>(piece, x, dout, act, row * cols, m, r, d, xh);
+            piece.load_vector(w, 1.f, wf);
 #pragma unroll
-            for (int e = 0; e < V; ++e) d[e] = r * (d[e] * wf[e] - c1 - xh[e] * c2);
-            store_chunk<T>(dx + row * cols + c, n, d);
+            for (int e = 0; e < V; ++e) d[e] = r * fmaf(-xh[e], c2, d[e] * wf[e] - c1);
+            piece.store(dx + row * cols, d);
         }
     }
 }
@@ -491,13 +629,13 @@ __global__ __launch_bounds__(256) void ln_bwd_long_dw_kernel(const T* __restrict
     constexpr int V = Elem<T>::CH;
     const int64_t c = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V;
     if (c >= cols) return;
-    const int n = cols - c < V ? (int)(cols - c) : V;
+    const Piece<T, int64_t, false> piece(c, cols);
     float dw[V], db[V], d[V], xh[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) dw[e] = db[e] = 0.f;
 #pragma unroll 4
     for (int64_t row = blockIdx.y; row < rows; row += gridDim.y) {
-        grad_chunk<T>(x, dout, act, row, c, cols, mean[row], rstd[row], d, xh);
+        grad_piece<T>(piece, x, dout, act, row * cols, mean[row], rstd[row], d, xh);
 #pragma unroll
         for (int e = 0; e < V; ++e) {
             db[e] += d[e];
@@ -506,9 +644,9 @@ __global__ __launch_bounds__(256) void ln_bwd_long_dw_kernel(const T* __restrict
     }
 #pragma unroll
     for (int e = 0; e < V; ++e)
-        if (e < n) {
-            partial[((int64_t)blockIdx.y * 2) * cols + c + e] = dw[e];
-            partial[((int64_t)blockIdx.y * 2 + 1) * cols + c + e] = db[e];
+        if (piece.own(e)) {
+            partial[((int64_t)blockIdx.y * 2) * cols + piece.from + e] = dw[e];
+            partial[((int64_t)blockIdx.y * 2 + 1) * cols + piece.from + e] = db[e];
         }
 }
 
@@ -516,16 +654,17 @@ __global__ __launch_bounds__(256) void ln_bwd_long_dw_kernel(const T* __restrict
 // Threads a row and chunks a thread, from the row's number of 16-byte chunks.  Up to 64 chunks: one a lane, the smallest power of two of
 // lanes (several rows share a wavefront).  Then a wavefront with up to KMAX a lane, then a workgroup of 256 .. 1024.  KMAX: what the
 // registers hold with four wavefronts a SIMD -- 4 forward; backward, which keeps a weight and two sums a column, 16 values (4 fp32
-// chunks, 2 bf16).
+// chunks, 2 bf16).  At 512 threads fp32 stops at 2: 16384 x 8192 takes 195 / 289 us forward / backward as 1024 threads of 2 chunks, 200 /
+// 309 as 512 of 4 (bf16, 8192 x 16384 forward: 107 against 99, the other way).
 struct Split { int tpr, k; };
-Split ln_split(int64_t chunks, int kmax) {
+Split ln_split(int dtype, int64_t chunks, int kmax) {
     if (chunks <= 64) {
         int tpr = 2;
         while (tpr < chunks) tpr *= 2;
         return {tpr, 1};
     }
     for (int tpr = 64; tpr <= 1024; tpr = tpr == 64 ? 256 : tpr * 2)
-        for (int k = 1; k <= kmax; k *= 2)
+        for (int k = 1; k <= (dtype == VINCE_F32 && tpr == 512 ? 2 : kmax); k *= 2)
             if ((int64_t)tpr * k >= chunks) return {tpr, k};
     return {0, 0};
 }
@@ -533,20 +672,36 @@ int ln_chunks(int dtype, int cols) { const int v = dtype == VINCE_F32 ? 4 : 8; r
 constexpr int LN_FWD_K = 4;
 constexpr int ln_bwd_k(int dtype) { return dtype == VINCE_F32 ? 4 : 2; }
 
-// Workgroups of the backward: at most two a CU -- each writes a partial row of 8 bytes a column that is read again -- and at least four
-// rows for each row group, so that the partial rows stay a small part of what is read anyway.
+// Workgroups: as many as have 4 MB of rows in their registers -- 2^18 chunks, of one tensor forward, of two backward -- and one a CU at
+// least; each goes through its share of the rows.  More rows at a time are slower, fewer too (forward, 65536 x 2048 bf16, us at 256 / 512
+// / 1024 / 2048 workgroups of 4 chunks a thread: 91 / 98 / 99 / 97; 10^6 x 128, of 1: 188 / 113 / 88 / 104; backward, 32768 x 4096, of 2:
+// 144 / 150 / 172 at 256 / 512 / 1024, where every workgroup also leaves a partial row of 8 bytes a column to be read again).
+int64_t ln_blocks(const Split& s, int64_t in_flight) {
+    const int64_t n = s.tpr ? in_flight / (block_threads(s.tpr) * s.k) : 1024;
+    return n < 256 ? 256 : n;
+}
+int64_t ln_fwd_blocks(int64_t rows, const Split& s) {
+    const int64_t r = s.tpr ? block_threads(s.tpr) / s.tpr : 1, want = (rows + r - 1) / r, most = ln_blocks(s, 1 << 18);
+    return want < most ? want : most;
+}
+// (at least four rows for each row group, so that the partial rows stay a small part of what is read)
 int ln_bwd_blocks(int64_t rows, const Split& s) {
-    const int64_t per = s.tpr == 0 ? 4 : 4 * (block_threads(s.tpr) / s.tpr);
+    const int64_t per = s.tpr ? 4 * (block_threads(s.tpr) / s.tpr) : 4, most = ln_blocks(s, 1 << 17);
     const int64_t n = (rows + per - 1) / per;
-    return (int)(n < 1 ? 1 : n > 512 ? 512 : n);
+    return (int)(n < 1 ? 1 : n > most ? most : n);
+}
+// Few rows (ln_bwd_few_kernel): one launch for two and no scratch, against reading x and dout twice and column sums that one workgroup makes
+// over all rows.  us of a call, two launches / one: 256 x 2048 fp32 8.4 / 5.3, 512 x 8192 bf16 14.7 / 9.9, 1024 x 512 fp32 8.1 / 5.7, 1024 x
+// 2048 bf16 9.0 / 10.0 (and 2 us for the scratch's allocation).
+bool ln_bwd_few(int dtype, int64_t rows, int cols, const Split& s) {
+    return s.tpr && rows <= 1024 && rows * ln_chunks(dtype, cols) <= (rows <= 512 ? 1 << 19 : 1 << 18);
 }
 
 template <typename T, int TPR, int K>
 void launch_fwd(const void* x, const float* w, const float* b, void* out, float* mean, float* rstd, int64_t rows, int cols, float eps, int relu,
                 hipStream_t st) {
-    constexpr int THREADS = block_threads(TPR), R = THREADS / TPR;
-    const int64_t want = (rows + R - 1) / R, most = 256 * 2048 / THREADS;
-    const dim3 grid((unsigned)(want < most ? want : most));
+    constexpr int THREADS = block_threads(TPR);
+    const dim3 grid((unsigned)ln_fwd_blocks(rows, {TPR, K}));
     if (cols == TPR * K * Elem<T>::CH)
         hipLaunchKernelGGL((ln_fwd_kernel<T, TPR, K, true>), grid, dim3(THREADS), 0, st, (const T*)x, w, b, (T*)out, mean, rstd, rows, cols, eps, relu);
     else
@@ -556,13 +711,15 @@ void launch_fwd(const void* x, const float* w, const float* b, void* out, float*
 template <typename T>
 void run_fwd(int dtype, const void* x, const float* w, const float* b, void* out, float* mean, float* rstd, int64_t rows, int cols, float eps,
              int relu, hipStream_t st) {
-    const Split s = ln_split(ln_chunks(dtype, cols), LN_FWD_K);
+    const Split s = ln_split(dtype, ln_chunks(dtype, cols), LN_FWD_K);
 #define LN_CASE(TPR, K) \
     if (s.tpr == TPR && s.k == K) return launch_fwd<T, TPR, K>(x, w, b, out, mean, rstd, rows, cols, eps, relu, st)
     LN_CASE(2, 1); LN_CASE(4, 1); LN_CASE(8, 1); LN_CASE(16, 1); LN_CASE(32, 1); LN_CASE(64, 1); LN_CASE(64, 2); LN_CASE(64, 4);
-    LN_CASE(256, 2); LN_CASE(256, 4); LN_CASE(512, 4); LN_CASE(1024, 4);
+    LN_CASE(256, 2); LN_CASE(256, 4); LN_CASE(1024, 4);
+    if constexpr (sizeof(T) == 4) { LN_CASE(1024, 2); }
+    else { LN_CASE(512, 4); }
 #undef LN_CASE
-    hipLaunchKernelGGL(ln_fwd_long_kernel<T>, dim3((unsigned)(rows < 1024 ? rows : 1024)), dim3(1024), 0, st, (const T*)x, w, b, (T*)out, mean, rstd,
+    hipLaunchKernelGGL(ln_fwd_long_kernel<T>, dim3((unsigned)ln_fwd_blocks(rows, s)), dim3(1024), 0, st, (const T*)x, w, b, (T*)out, mean, rstd,
                        rows, cols, eps, relu);
 }
 
@@ -570,18 +727,30 @@ struct BwdArgs {
     const void *x, *dout, *act;
     const float *w, *mean, *rstd;
     void* dx;
-    float *dw, *db, *partial;
+    float *dw, *db, *partial;      // partial == NULL with dw: few rows, one launch
     int accumulate;
     int64_t rows;
     int cols, blocks;
 };
 
 template <typename T, int TPR, int K> void launch_bwd(const BwdArgs& a, hipStream_t st) {
-    const bool full = a.cols == TPR * K * Elem<T>::CH;
-#define LN_LAUNCH(FULL, ACT)                                                                                                              \
-    if (full == FULL && (a.act != nullptr) == ACT)                                                                                        \
-        hipLaunchKernelGGL((ln_bwd_kernel<T, TPR, K, FULL, ACT>), dim3(a.blocks), dim3(block_threads(TPR)), 0, st, (const T*)a.x, a.w, a.mean, \
-                           a.rstd, (const T*)a.dout, (const T*)a.act, (T*)a.dx, a.dw, a.db, a.accumulate, a.partial, a.rows, a.cols)
+    constexpr int THREADS = block_threads(TPR), R = THREADS / TPR, V = Elem<T>::CH;
+    if (a.dw && !a.partial) {
+        const int dx_blocks = (int)((a.rows + R - 1) / R), dw_blocks = (a.cols + 8 * V - 1) / (8 * V);
+#define LN_LAUNCH(ACT)                                                                                                                        \
+    if ((a.act != nullptr) == ACT)                                                                                                            \
+    hipLaunchKernelGGL((ln_bwd_few_kernel<T, TPR, K, ACT>), dim3(dx_blocks + dw_blocks), dim3(THREADS), 0, st, (const T*)a.x, a.w, a.mean, a.rstd, \
+                       (const T*)a.dout, (const T*)a.act, (T*)a.dx, a.dw, a.db, a.accumulate, (int)a.rows, a.cols, dx_blocks)
+        LN_LAUNCH(false);
+        LN_LAUNCH(true);
+#undef LN_LAUNCH
+        return;
+    }
+    const bool full = a.cols == TPR * K * V;
+#define LN_LAUNCH(FULL, ACT)                                                                                                               \
+    if (full == FULL && (a.act != nullptr) == ACT)                                                                                         \
+    hipLaunchKernelGGL((ln_bwd_kernel<T, TPR, K, FULL, ACT>), dim3(a.blocks), dim3(THREADS), 0, st, (const T*)a.x, a.w, a.mean, a.rstd,    \
+                       (const T*)a.dout, (const T*)a.act, (T*)a.dx, a.partial, a.rows, a.cols)
     LN_LAUNCH(true, false);
     LN_LAUNCH(true, true);
     LN_LAUNCH(false, false);
@@ -594,7 +763,7 @@ template <typename T> void run_bwd(const Split& s, const BwdArgs& a, hipStream_t
     if (s.tpr == TPR && s.k == K) return launch_bwd<T, TPR, K>(a, st)
     LN_CASE(2, 1); LN_CASE(4, 1); LN_CASE(8, 1); LN_CASE(16, 1); LN_CASE(32, 1); LN_CASE(64, 1); LN_CASE(64, 2); LN_CASE(256, 2);
     if constexpr (sizeof(T) == 4) {
-        LN_CASE(64, 4); LN_CASE(256, 4); LN_CASE(512, 4); LN_CASE(1024, 4);
+        LN_CASE(64, 4); LN_CASE(256, 4); LN_CASE(1024, 2); LN_CASE(1024, 4);
     } else {
         LN_CASE(256, 1); LN_CASE(512, 2); LN_CASE(1024, 2);
     }
@@ -626,9 +795,8 @@ extern "C" int vince_layer_norm_fwd(int dtype, const void* x, const float* weigh
 
 extern "C" size_t vince_layer_norm_bwd_scratch_bytes(int dtype, int64_t rows, int32_t cols) {
     if (rows <= 0 || cols <= 0) return 0;
-    const Split s = ln_split(ln_chunks(dtype, cols), ln_bwd_k(dtype));
-    const int blocks = ln_bwd_blocks(rows, s);
-    return blocks == 1 && s.tpr ? 0 : (size_t)blocks * 2 * (size_t)cols * sizeof(float);
+    const Split s = ln_split(dtype, ln_chunks(dtype, cols), ln_bwd_k(dtype));
+    return ln_bwd_few(dtype, rows, cols, s) ? 0 : (size_t)ln_bwd_blocks(rows, s) * 2 * (size_t)cols * sizeof(float);
 }
 
 extern "C" int vince_layer_norm_bwd(int dtype, const void* x, const float* weight, const float* mean, const float* rstd, const void* dout,
@@ -637,19 +805,19 @@ extern "C" int vince_layer_norm_bwd(int dtype, const void* x, const float* weigh
     LN_CHECK("vince_layer_norm_bwd");
     VINCE_CHECK_ARG((dweight == nullptr) == (dbias == nullptr), VINCE_E_ARG, "vince_layer_norm_bwd: dweight and dbias come together");
     hipStream_t st = (hipStream_t)stream;
-    const Split s = ln_split(ln_chunks(dtype, cols), ln_bwd_k(dtype));
+    const Split s = ln_split(dtype, ln_chunks(dtype, cols), ln_bwd_k(dtype));
     const int blocks = ln_bwd_blocks(rows, s);
-    const bool direct = rows > 0 && blocks == 1 && s.tpr;       // one workgroup: it writes dweight and dbias itself
+    const bool few = rows > 0 && ln_bwd_few(dtype, rows, cols, s);
     if (rows > 0) {
         VINCE_CHECK_ARG(x && mean && rstd && dout && dx, VINCE_E_ARG, "vince_layer_norm_bwd: null pointer");
         const size_t need = dweight ? vince_layer_norm_bwd_scratch_bytes(dtype, rows, cols) : 0;
         VINCE_CHECK_ARG(need == 0 || (scratch && scratch_bytes >= need), VINCE_E_ARG, "vince_layer_norm_bwd: scratch of %zu bytes", scratch_bytes);
-        const BwdArgs a = {x, dout, act, weight, mean, rstd, dx, dweight, dbias, direct ? nullptr : (float*)scratch, accumulate, rows, cols, blocks};
+        const BwdArgs a = {x, dout, act, weight, mean, rstd, dx, dweight, dbias, few || !dweight ? nullptr : (float*)scratch, accumulate, rows, cols, blocks};
         if (dtype == VINCE_F32) run_bwd<float>(s, a, st);
         else run_bwd<bf16_t>(s, a, st);
         VINCE_CHECK_LAUNCH();
     }
-    if (dweight && !direct && (rows > 0 || !accumulate)) {
+    if (dweight && !few && (rows > 0 || !accumulate)) {
         hipLaunchKernelGGL(ln_bwd_join_kernel, dim3((unsigned)((2 * (int64_t)cols + 31) / 32)), dim3(1024), 0, st, (const float*)scratch,
                            rows > 0 ? blocks : 0, 2 * (int64_t)cols, cols, dweight, dbias, accumulate);
         VINCE_CHECK_LAUNCH();

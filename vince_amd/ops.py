@@ -45,18 +45,13 @@ def require_gpu(*tensors):
 
 
 def _one_gpu(*tensors):
-    """The device that every given tensor (None: not given) is on; contiguous GPU tensors only."""
-    dev = None
+    """The index of the one device that every given tensor (None: not given) is on; contiguous GPU tensors only."""
+    index = tensors[0].get_device()
     for t in tensors:
-        if t is None:
-            continue
-        if not t.is_cuda or not t.is_contiguous():
-            require_gpu(t)
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise RuntimeError("vince_amd: tensors on %s and %s -- one call works on one GPU" % (dev, t.device))
-    return dev
+        if t is not None and (t.get_device() != index or not t.is_contiguous() or index < 0):
+            require_gpu(*tensors)
+            raise RuntimeError("vince_amd: tensors on %s and %s -- one call works on one GPU" % (tensors[0].device, t.device))
+    return index
 
 
 def _raw_stream(index):
@@ -64,14 +59,15 @@ def _raw_stream(index):
     return torch._C._cuda_getCurrentRawStream(index)
 
 
-def _launch(dev, fn, *args):
-    """fn(*args, stream) on the current stream of `dev`, whichever device is current."""
-    index = dev.index
-    if index == torch.cuda.current_device():
-        check(fn(*args, _raw_stream(index)))
+def _launch(index, fn, *args):
+    """fn(*args, stream) on the current stream of device `index`, whichever device is current."""
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):
-            check(fn(*args, _raw_stream(index)))
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc != 0:
+        check(rc)
 
 
 # ------------------------------------------------------------------------------------------------ conv descriptors
@@ -387,31 +383,35 @@ def l2norm_bwd(x, norms, dout, eps=1e-12):
 
 
 # ------------------------------------------------------------------------------------------------ batch norm / pooling
-def _layer_norm_vectors(what, cols, **vectors):
-    for name, v in vectors.items():
-        if v is not None and (v.dtype != torch.float32 or v.shape != (cols,)):
-            raise ValueError("%s: %s has to be float32 [%d], got %s %s" % (what, name, cols, v.dtype, tuple(v.shape)))
+def _layer_norm_shape(what, x):
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise ValueError("%s: x has no last axis to normalise, got shape %s" % (what, tuple(x.shape)))
+    return dtype_code(x), x.shape[-1]
+
+
+def _layer_norm_vector(what, name, v, cols):
+    if v.dtype != torch.float32 or v.dim() != 1 or v.numel() != cols:
+        raise ValueError("%s: %s has to be float32 [%d], got %s %s" % (what, name, cols, v.dtype, tuple(v.shape)))
+    return v.data_ptr()
 
 
 def layer_norm_fwd(x, weight=None, bias=None, eps=1e-5, relu=False):
     """Layer norm over the last axis of x [..., D] (float32 or bfloat16): (x - mean) * rstd * weight + bias, rstd = 1 / sqrt(var + eps)
     with the biased variance; relu: max(., 0) in the same pass.  weight, bias: float32 [D] or None (no bias without a weight).
     Returns (out like x, mean float32 [...], rstd float32 [...]); layer_norm_bwd takes the last two."""
-    dev = _one_gpu(x, weight, bias)
-    code = dtype_code(x)
-    if x.dim() == 0 or x.shape[-1] == 0:
-        raise ValueError("layer_norm_fwd: x has no last axis to normalise, got shape %s" % (tuple(x.shape),))
+    index = _one_gpu(x, weight, bias)
+    code, cols = _layer_norm_shape("layer_norm_fwd", x)
     if weight is None and bias is not None:
         raise ValueError("layer_norm_fwd: a bias without a weight")
     if not eps >= 0:
         raise ValueError("layer_norm_fwd: eps=%r" % (eps,))
-    cols = x.shape[-1]
-    _layer_norm_vectors("layer_norm_fwd", cols, weight=weight, bias=bias)
+    w = None if weight is None else _layer_norm_vector("layer_norm_fwd", "weight", weight, cols)
+    b = None if bias is None else _layer_norm_vector("layer_norm_fwd", "bias", bias, cols)
     out = torch.empty_like(x)
-    mean = torch.empty(x.shape[:-1], device=dev, dtype=torch.float32)
+    mean = x.new_empty(x.shape[:-1], dtype=torch.float32)
     rstd = torch.empty_like(mean)
-    _launch(dev, lib().vince_layer_norm_fwd, code, x.data_ptr(), None if weight is None else weight.data_ptr(),
-            None if bias is None else bias.data_ptr(), out.data_ptr(), mean.data_ptr(), rstd.data_ptr(), mean.numel(), cols, eps, int(relu))
+    _launch(index, lib().vince_layer_norm_fwd, code, x.data_ptr(), w, b, out.data_ptr(), mean.data_ptr(), rstd.data_ptr(), mean.numel(),
+            cols, eps, bool(relu))
     return out, mean, rstd
 
 
@@ -420,30 +420,31 @@ def layer_norm_bwd(x, weight, mean, rstd, dout, act=None, dweight=None, dbias=No
     act: the output of a forward with relu=True -- dout counts as zero where act <= 0 (as ops.relu_bwd has it).
     dweight, dbias: float32 [D] buffers the parameters' gradients are ADDED to (as ops.linear_bwd does); without them they are returned
     in new tensors.  Without a weight there are neither.  Returns (dx, dweight, dbias).  Same bits on every call: no atomics."""
-    dev = _one_gpu(x, weight, mean, rstd, dout, act, dweight, dbias)
-    code = dtype_code(x)
-    if x.dim() == 0 or x.shape[-1] == 0:
-        raise ValueError("layer_norm_bwd: x has no last axis, got shape %s" % (tuple(x.shape),))
+    index = _one_gpu(x, weight, mean, rstd, dout, act, dweight, dbias)
+    code, cols = _layer_norm_shape("layer_norm_bwd", x)
     for name, t in (("dout", dout), ("act", act)):
         if t is not None and (t.dtype != x.dtype or t.shape != x.shape):
             raise ValueError("layer_norm_bwd: %s is %s %s, x is %s %s" % (name, t.dtype, tuple(t.shape), x.dtype, tuple(x.shape)))
-    cols = x.shape[-1]
+    rows = mean.numel()
     for name, t in (("mean", mean), ("rstd", rstd)):
         if t.dtype != torch.float32 or t.numel() * cols != x.numel():
             raise ValueError("layer_norm_bwd: %s has to hold one float32 per row of x, got %s %s" % (name, t.dtype, tuple(t.shape)))
     if (dweight is None) != (dbias is None) or (weight is None and dweight is not None):
         raise ValueError("layer_norm_bwd: dweight and dbias come together, and with a weight")
-    _layer_norm_vectors("layer_norm_bwd", cols, weight=weight, dweight=dweight, dbias=dbias)
-    accumulate = dweight is not None
-    if weight is not None and not accumulate:
-        dweight, dbias = torch.empty_like(weight), torch.empty_like(weight)
-    rows = mean.numel()
     dx = torch.empty_like(x)
-    nbytes = 0 if weight is None else lib().vince_layer_norm_bwd_scratch_bytes(code, rows, cols)
-    scratch = torch.empty(nbytes, device=dev, dtype=torch.uint8) if nbytes else None
-    _launch(dev, lib().vince_layer_norm_bwd, code, x.data_ptr(), None if weight is None else weight.data_ptr(), mean.data_ptr(),
-            rstd.data_ptr(), dout.data_ptr(), None if act is None else act.data_ptr(), dx.data_ptr(),
-            None if dweight is None else dweight.data_ptr(), None if dbias is None else dbias.data_ptr(), int(accumulate), rows, cols,
+    w = dw = db = scratch = None
+    nbytes, accumulate = 0, dweight is not None
+    if weight is not None:
+        w = _layer_norm_vector("layer_norm_bwd", "weight", weight, cols)
+        if not accumulate:
+            dweight, dbias = torch.empty_like(weight), torch.empty_like(weight)
+        dw = _layer_norm_vector("layer_norm_bwd", "dweight", dweight, cols)
+        db = _layer_norm_vector("layer_norm_bwd", "dbias", dbias, cols)
+        nbytes = lib().vince_layer_norm_bwd_scratch_bytes(code, rows, cols)
+        if nbytes:
+            scratch = x.new_empty(nbytes, dtype=torch.uint8)      # (a call's own: two may be in flight)
+    _launch(index, lib().vince_layer_norm_bwd, code, x.data_ptr(), w, mean.data_ptr(), rstd.data_ptr(), dout.data_ptr(),
+            None if act is None else act.data_ptr(), dx.data_ptr(), dw, db, accumulate, rows, cols,
             None if scratch is None else scratch.data_ptr(), nbytes)
     return dx, dweight, dbias
 
@@ -761,13 +762,13 @@ def ema_flat(key, query, momentum):
 def sgd_flat(param, grad, buf, lr, momentum=0.9, weight_decay=1e-4, grad_scale=1.0, clip=None):
     """clip: what grad_norm returned -- the gradient is scaled by clip[1] too, without being rewritten."""
     if clip is not None:
-        dev = _one_gpu(param, grad, buf, clip)
+        index = _one_gpu(param, grad, buf, clip)
         if not (param.dtype == grad.dtype == buf.dtype == clip.dtype == torch.float32) or clip.numel() != 2:
             raise TypeError("vince_amd: sgd_flat takes float32 tensors, and a clip of two values (grad_norm)")
         if not param.numel() == grad.numel() == buf.numel():
             raise ValueError("vince_amd: sgd_flat: %d parameters, %d gradients, %d momentum values"
                              % (param.numel(), grad.numel(), buf.numel()))
-        _launch(dev, lib().vince_sgd_flat_clip, param.data_ptr(), grad.data_ptr(), buf.data_ptr(), param.numel(), lr, momentum, weight_decay,
+        _launch(index, lib().vince_sgd_flat_clip, param.data_ptr(), grad.data_ptr(), buf.data_ptr(), param.numel(), lr, momentum, weight_decay,
                 grad_scale, clip.data_ptr())
         return
     require_gpu(param, grad, buf)
@@ -825,12 +826,13 @@ class GradTable:
         check(lib().vince_grad_table_fill(entries, len(self.tensors), host.data_ptr(), self.chunks))
         self._table = host.to(self.device)            # (synchronous: any stream may read it from here on)
         self._scratch_bytes = lib().vince_grad_norm_scratch_bytes(self.chunks)
-        self._stream = _raw_stream(self.device.index)
+        self._index, self._ptr = self.device.index, self._table.data_ptr()
+        self._stream = _raw_stream(self._index)
 
     def _run(self, fn, *args):
-        if _raw_stream(self.device.index) != self._stream:     # (its memory outlives what another stream still has to read)
+        if _raw_stream(self._index) != self._stream:     # (its memory outlives what another stream still has to read)
             self._table.record_stream(torch.cuda.current_stream(self.device))
-        _launch(self.device, fn, self._table.data_ptr(), self.chunks, *args)
+        _launch(self._index, fn, self._ptr, self.chunks, *args)
 
     def _norm(self, fn, max_norm):
         max_norm = float("inf") if max_norm is None else float(max_norm)
@@ -861,7 +863,7 @@ def grad_clip(grads, max_norm):
 def grad_scale(grads, clip):
     """Every gradient times clip[1], in place: for gradients that another call's norm includes."""
     table = _grad_table(grads)
-    if _one_gpu(clip) != table.device or clip.dtype != torch.float32 or clip.numel() != 2:
+    if _one_gpu(clip) != table.device.index or clip.dtype != torch.float32 or clip.numel() != 2:
         raise ValueError("grad_scale: clip is what grad_norm returns (float32 [2]) on %s" % (table.device,))
     table._run(lib().vince_grad_scale, clip.data_ptr())
 
