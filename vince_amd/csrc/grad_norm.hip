@@ -1,12 +1,17 @@
 // The 2-norm over many gradient tensors, clipping to a largest norm, and the SGD step that takes the clipping coefficient from device
-// memory (include/vince_hip.h has the formulas).  A table in device memory lists the tensors in pieces of at most GRAD_CHUNK elements.
+// memory (include/vince_hip.h has the formulas).  A table in device memory lists the tensors in pieces of a few thousand elements.
 // Squares of fp32 / bf16 values are exact in fp64 and their fp64 sum neither overflows nor underflows, whatever the gradients' scale.
 #include "common.h"
 
 namespace {
 
-constexpr int GRAD_CHUNK = 16384;
-constexpr int GRAD_BLOCKS = 1024;      // 4 workgroups a CU
+// Pieces of 2048 .. 16384 elements: small enough that a few hundred thousand elements reach every CU, large enough that the entries are
+// nothing beside what they list.
+constexpr int GRAD_CHUNK_MIN = 2048, GRAD_CHUNK_MAX = 16384;
+// Workgroups: 8 MB of loads in flight where only gradients are read, 4 MB where they are written back too, 3 MB in the SGD step's three
+// streams.  us at 256 / 512 / 1024 / 2048 of them, 160 M fp32: norm 126 / 103 / 107 / 112 (6.2 TB/s at 512), scaling 219 / 244 / 246 / 247,
+// SGD step 593 / 605 / 668 / 690.  (A piece's entry is read when the piece begins: read ahead, scaling takes 247 us at 256, norm 107 at 512.)
+constexpr int GRAD_NORM_BLOCKS = 512, GRAD_SCALE_BLOCKS = 256, SGD_BLOCKS = 256;
 constexpr uint32_t GRAD_BF16 = 1u << 31;
 
 struct GradChunk {
@@ -134,7 +139,7 @@ template <typename T> __device__ __forceinline__ void scale_piece(T* __restrict_
     }
 }
 
-// FINAL: the coefficient comes from the sums of grad_squares_kernel, added up by every workgroup for itself (8 KB at most, in the
+// FINAL: the coefficient comes from the sums of grad_squares_kernel, added up by every workgroup for itself (4 KB at most, in the
 // caches) -- one launch fewer than a kernel of its own for it; else from clip[1]
 template <bool FINAL>
 __global__ __launch_bounds__(256) void grad_scale_kernel(const GradChunk* __restrict__ table, int64_t chunks, float* __restrict__ clip,
@@ -182,7 +187,13 @@ __global__ __launch_bounds__(256) void sgd_clip_kernel(float* __restrict__ p, co
     }
 }
 
-int grad_blocks(int64_t chunks) { return (int)(chunks < GRAD_BLOCKS ? chunks : GRAD_BLOCKS); }
+int blocks_of(int64_t chunks, int most) { return (int)(chunks < most ? chunks : most); }
+int64_t chunk_of(const vince_grad_tensor* tensors, int32_t count) {
+    int64_t total = 0, chunk = GRAD_CHUNK_MIN;
+    for (int32_t i = 0; i < count; ++i) total += tensors[i].n;
+    while (chunk < GRAD_CHUNK_MAX && chunk * 2 * GRAD_NORM_BLOCKS <= total) chunk *= 2;
+    return chunk;
+}
 
 }  // namespace
 
@@ -196,8 +207,9 @@ extern "C" int64_t vince_grad_table_chunks(const vince_grad_tensor* tensors, int
         VINCE_CHECK_ARG(t.n >= 0 && (t.data || t.n == 0), VINCE_E_ARG, "vince_grad_table: tensor %d: n=%lld", i, (long long)t.n);
         VINCE_CHECK_ARG(((uintptr_t)t.data & (t.dtype == VINCE_F32 ? 3 : 1)) == 0, VINCE_E_ALIGN, "vince_grad_table: tensor %d is not aligned to its elements", i);
         VINCE_CHECK_ARG(t.scale - t.scale == 0.f, VINCE_E_ARG, "vince_grad_table: tensor %d: scale %g", i, (double)t.scale);
-        chunks += t.n / GRAD_CHUNK + (t.n % GRAD_CHUNK != 0);
     }
+    const int64_t chunk = chunk_of(tensors, count);
+    for (int32_t i = 0; i < count; ++i) chunks += tensors[i].n / chunk + (tensors[i].n % chunk != 0);
     return chunks;
 }
 
@@ -206,19 +218,20 @@ extern "C" int vince_grad_table_fill(const vince_grad_tensor* tensors, int32_t c
     if (want < 0) return (int)want;
     VINCE_CHECK_ARG(chunks == want && (table || chunks == 0), VINCE_E_ARG, "vince_grad_table_fill: %lld entries, not %lld", (long long)chunks, (long long)want);
     GradChunk* c = (GradChunk*)table;
+    const int64_t chunk = chunk_of(tensors, count);
     for (int32_t i = 0; i < count; ++i) {
         const vince_grad_tensor& t = tensors[i];
         const uint64_t size = t.dtype == VINCE_F32 ? 4 : 2;
-        for (int64_t at = 0; at < t.n; at += GRAD_CHUNK, ++c) {
+        for (int64_t at = 0; at < t.n; at += chunk, ++c) {
             c->data = (uint64_t)(uintptr_t)t.data + (uint64_t)at * size;
-            c->n = (uint32_t)(t.n - at < GRAD_CHUNK ? t.n - at : GRAD_CHUNK) | (t.dtype == VINCE_BF16 ? GRAD_BF16 : 0u);
+            c->n = (uint32_t)(t.n - at < chunk ? t.n - at : chunk) | (t.dtype == VINCE_BF16 ? GRAD_BF16 : 0u);
             c->scale = t.scale;
         }
     }
     return VINCE_OK;
 }
 
-extern "C" size_t vince_grad_norm_scratch_bytes(int64_t chunks) { return chunks > 0 ? (size_t)grad_blocks(chunks) * sizeof(double) : 0; }
+extern "C" size_t vince_grad_norm_scratch_bytes(int64_t chunks) { return chunks > 0 ? (size_t)blocks_of(chunks, GRAD_NORM_BLOCKS) * sizeof(double) : 0; }
 
 #define GRAD_NORM_CHECK(name)                                                                                                              \
     VINCE_CHECK_ARG(chunks >= 0 && clip && (chunks == 0 || (table && scratch)), VINCE_E_ARG, name ": bad arguments");                      \
@@ -227,7 +240,7 @@ extern "C" size_t vince_grad_norm_scratch_bytes(int64_t chunks) { return chunks 
 
 extern "C" int vince_grad_norm(const void* table, int64_t chunks, float max_norm, float* clip, void* scratch, size_t scratch_bytes, void* stream) {
     GRAD_NORM_CHECK("vince_grad_norm");
-    const int blocks = grad_blocks(chunks);
+    const int blocks = blocks_of(chunks, GRAD_NORM_BLOCKS);
     if (blocks > 0)
         hipLaunchKernelGGL(grad_squares_kernel, dim3(blocks), dim3(256), 0, (hipStream_t)stream, (const GradChunk*)table, chunks, (double*)scratch);
     hipLaunchKernelGGL(grad_clip_kernel, dim3(1), dim3(256), 0, (hipStream_t)stream, (const double*)scratch, blocks, max_norm, clip);
@@ -238,7 +251,7 @@ extern "C" int vince_grad_norm(const void* table, int64_t chunks, float max_norm
 extern "C" int vince_grad_scale(const void* table, int64_t chunks, const float* clip, void* stream) {
     VINCE_CHECK_ARG(chunks >= 0 && clip && (chunks == 0 || table), VINCE_E_ARG, "vince_grad_scale: bad arguments");
     if (chunks == 0) return VINCE_OK;
-    hipLaunchKernelGGL(grad_scale_kernel<false>, dim3(grad_blocks(chunks)), dim3(256), 0, (hipStream_t)stream, (const GradChunk*)table, chunks,
+    hipLaunchKernelGGL(grad_scale_kernel<false>, dim3(blocks_of(chunks, GRAD_SCALE_BLOCKS)), dim3(256), 0, (hipStream_t)stream, (const GradChunk*)table, chunks,
                        (float*)clip, (const double*)nullptr, 0, 0.f);
     VINCE_CHECK_LAUNCH();
     return VINCE_OK;
@@ -247,9 +260,9 @@ extern "C" int vince_grad_scale(const void* table, int64_t chunks, const float* 
 extern "C" int vince_grad_clip(const void* table, int64_t chunks, float max_norm, float* clip, void* scratch, size_t scratch_bytes, void* stream) {
     GRAD_NORM_CHECK("vince_grad_clip");
     if (chunks == 0) return vince_grad_norm(table, chunks, max_norm, clip, scratch, scratch_bytes, stream);
-    const int blocks = grad_blocks(chunks);
+    const int blocks = blocks_of(chunks, GRAD_NORM_BLOCKS);
     hipLaunchKernelGGL(grad_squares_kernel, dim3(blocks), dim3(256), 0, (hipStream_t)stream, (const GradChunk*)table, chunks, (double*)scratch);
-    hipLaunchKernelGGL(grad_scale_kernel<true>, dim3(blocks), dim3(256), 0, (hipStream_t)stream, (const GradChunk*)table, chunks, clip,
+    hipLaunchKernelGGL(grad_scale_kernel<true>, dim3(blocks_of(chunks, GRAD_SCALE_BLOCKS)), dim3(256), 0, (hipStream_t)stream, (const GradChunk*)table, chunks, clip,
                        (const double*)scratch, blocks, max_norm);
     VINCE_CHECK_LAUNCH();
     return VINCE_OK;
@@ -261,7 +274,7 @@ extern "C" int vince_sgd_flat_clip(float* param, const float* grad, float* buf, 
     VINCE_CHECK_ARG((((uintptr_t)param | (uintptr_t)grad | (uintptr_t)buf) & 15) == 0, VINCE_E_ALIGN,
                     "vince_sgd_flat_clip: pointers must be 16-byte aligned");
     const int64_t blocks = (n / 4 + 256) / 256;
-    hipLaunchKernelGGL(sgd_clip_kernel, dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, (hipStream_t)stream, param, grad, buf, n, lr,
+    hipLaunchKernelGGL(sgd_clip_kernel, dim3((unsigned)(blocks < SGD_BLOCKS ? blocks : SGD_BLOCKS)), dim3(256), 0, (hipStream_t)stream, param, grad, buf, n, lr,
                        momentum, weight_decay, grad_scale, clip);
     VINCE_CHECK_LAUNCH();
     return VINCE_OK;
