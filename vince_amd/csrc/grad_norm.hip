@@ -8,10 +8,11 @@ namespace {
 // Pieces of 2048 .. 16384 elements: small enough that a few hundred thousand elements reach every CU, large enough that the entries are
 // nothing beside what they list.
 constexpr int GRAD_CHUNK_MIN = 2048, GRAD_CHUNK_MAX = 16384;
-// Workgroups: 8 MB of loads in flight where only gradients are read, 4 MB where they are written back too, 3 MB in the SGD step's three
-// streams.  us at 256 / 512 / 1024 / 2048 of them, 160 M fp32: norm 126 / 103 / 107 / 112 (6.2 TB/s at 512), scaling 219 / 244 / 246 / 247,
-// SGD step 593 / 605 / 668 / 690.  (A piece's entry is read when the piece begins: read ahead, scaling takes 247 us at 256, norm 107 at 512.)
-constexpr int GRAD_NORM_BLOCKS = 512, GRAD_SCALE_BLOCKS = 256, SGD_BLOCKS = 256;
+// Workgroups: 8 MB of loads in flight where only gradients are read, 4 MB where they are written back too, 6 MB in the SGD step's three
+// streams.  us at 256 / 512 / 1024 / 2048 of them, 160 M fp32: norm 126 / 103 / 107 / 112 (6.2 TB/s at 512), scaling 219 / 244 / 246 / 247;
+// norm and SGD step of 28 M at 256 / 512: 120 / 112.  (A piece's entry is read when the piece begins: read ahead, scaling takes 247 us at
+// 256, the norm 107 at 512.)
+constexpr int GRAD_NORM_BLOCKS = 512, GRAD_SCALE_BLOCKS = 256, SGD_BLOCKS = 512;
 constexpr uint32_t GRAD_BF16 = 1u << 31;
 
 struct GradChunk {
@@ -161,7 +162,11 @@ __global__ __launch_bounds__(256) void grad_scale_kernel(const GradChunk* __rest
     }
 }
 
-// sgd_kernel (misc.hip) with the scale of the gradient taken from device memory: the same operations in the same order
+// sgd_kernel (misc.hip) with the scale of the gradient taken from device memory: the same operations in the same order.  The momentum
+// passes the Infinity Cache by (non-temporal both ways; nothing reads it before the next step), which leaves the gradients there that the
+// norm has just read, and the parameters for the average and the weight copies that follow: norm and step of 28 M parameters 122 -> 112 us,
+// with the key encoder's average behind them 175 -> 166.
+typedef __attribute__((ext_vector_type(4))) float f32x4_nt_t;
 __global__ __launch_bounds__(256) void sgd_clip_kernel(float* __restrict__ p, const float* __restrict__ g, float* __restrict__ buf, int64_t n,
                                                        float lr, float mom, float wd, float grad_scale, const float* __restrict__ clip) {
     const float gs = grad_scale * clip[1];
@@ -169,14 +174,16 @@ __global__ __launch_bounds__(256) void sgd_clip_kernel(float* __restrict__ p, co
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n4; i += (int64_t)gridDim.x * 256) {
         float4 pv = ((float4*)p)[i];
         const float4 gv = ((const float4*)g)[i];
-        float4 bv = ((float4*)buf)[i];
+        f32x4_nt_t bq = __builtin_nontemporal_load((const f32x4_nt_t*)buf + i);
+        float4 bv = make_float4(bq[0], bq[1], bq[2], bq[3]);
         float d;
         d = fmaf(wd, pv.x, gv.x * gs); bv.x = fmaf(bv.x, mom, d); pv.x = fmaf(-lr, bv.x, pv.x);
         d = fmaf(wd, pv.y, gv.y * gs); bv.y = fmaf(bv.y, mom, d); pv.y = fmaf(-lr, bv.y, pv.y);
         d = fmaf(wd, pv.z, gv.z * gs); bv.z = fmaf(bv.z, mom, d); pv.z = fmaf(-lr, bv.z, pv.z);
         d = fmaf(wd, pv.w, gv.w * gs); bv.w = fmaf(bv.w, mom, d); pv.w = fmaf(-lr, bv.w, pv.w);
         ((float4*)p)[i] = pv;
-        ((float4*)buf)[i] = bv;
+        bq = (f32x4_nt_t){bv.x, bv.y, bv.z, bv.w};
+        __builtin_nontemporal_store(bq, (f32x4_nt_t*)buf + i);
     }
     if (blockIdx.x == 0 && threadIdx.x < (n & 3)) {
         const int64_t i = (n4 << 2) + threadIdx.x;
