@@ -46,9 +46,10 @@ template <typename T> __device__ __forceinline__ void store_few(T* __restrict__ 
         }
 }
 
-// The chunk that starts at column `col` of a row of `cols`.  One that the row's end cuts is taken as the row's last 16 bytes: one load
-// and one store whatever it holds, nothing to shift; its first elements are the chunk's before it, and stay out of the sums (own()).
-// A chunk behind the row's end reads the row's last 16 bytes too, and owns nothing.  SHORT: the row may have less than 16 bytes.
+// The chunk of columns col .. col + V - 1 of a row of `cols`; col may be below 0, the chunk may reach past the row's end or lie outside.
+// One that the row does not fill is taken as the 16 bytes of the row that are nearest: one load and one store whatever it holds, nothing
+// to shift; the elements outside its own columns are its neighbour's, and stay out of the sums (own()).  SHORT: the row may have less than
+// 16 bytes (then col >= 0).
 template <typename T, typename I, bool SHORT> struct Piece {
     static constexpr int V = Elem<T>::CH;
     I from;
@@ -57,11 +58,11 @@ template <typename T, typename I, bool SHORT> struct Piece {
         const bool small = SHORT && cols_ < V;
         cols = small ? (int)cols_ : V;
         const I last = small ? 0 : cols_ - V;
-        from = col < last ? col : last;
-        first = (int)(col - from < V ? col - from : V);
-        n = small ? (col == 0 ? (int)cols_ : 0) : V - first;
+        from = col < 0 ? 0 : col < last ? col : last;
+        first = (int)(col < from ? 0 : col - from < V ? col - from : V);
+        n = small ? (col == 0 ? (int)cols_ : 0) : col < 0 ? (int)(col + V) : V - first;
     }
-    __device__ __forceinline__ bool own(int e) const { return SHORT ? (unsigned)(e - first) < (unsigned)n : e >= first; }
+    __device__ __forceinline__ bool own(int e) const { return (unsigned)(e - first) < (unsigned)n; }
     __device__ __forceinline__ uint4 load(const T* __restrict__ row) const {
         if (SHORT && cols < V) return load_few<T>(row, cols);
         return load16<T>(row + from);
@@ -112,8 +113,12 @@ template <int N> __device__ __forceinline__ float strided_sum(float v) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// TPR, threads a row: up to 64 exactly, in workgroups of 256; more than 64, the most of a row's own workgroup, which has as many
+// wavefronts (blockDim.x / 64, 16 at most) as the row needs.
 constexpr int block_threads(int tpr) { return tpr > 64 ? tpr : 256; }
 constexpr int wave_lanes(int tpr) { return tpr < 64 ? tpr : 64; }
+// the sum of a workgroup's per-wavefront values, one in each of 16 neighbouring lanes (0 behind the last wavefront)
+__device__ __forceinline__ float waves_sum(float v) { return lanes_sum<16>(v); }
 // Whether a thread keeps its columns' weight (and bias) in registers from row to row.  At 1024 threads, with 128 registers each, there is
 // room for 8 values only: else they are read again for every row, from the caches.
 constexpr bool holds_weights(int tpr, int values) { return tpr < 1024 || values <= 8; }
@@ -125,14 +130,24 @@ __device__ __forceinline__ float divide(float s, float n, float inv) {
     return better == better ? better : q;          // (an infinite sum: the correction is NaN)
 }
 
-// This thread's K chunks of a row.  FULL: cols == TPR * K * V, every chunk whole.  Else the first K / 2 are (ln_split takes K > 1 for rows
-// of more than TPR * K / 2 chunks).
-template <typename T, int TPR, int K, bool FULL> struct Cols {
+// How the rows lie.  FULL: cols == TPR * K * V, every chunk whole.  PLAIN: the chunks start with the row, the first K / 2 are whole
+// (ln_split takes K > 1 for rows of more than TPR * K / 2 chunks).  SHIFTED: bfloat16 rows of an odd length start at every other address;
+// a 16-byte access that is not even aligned to 4 bytes occupies the vector cache three times as long (PMC: 49 M accesses for 15 M in the
+// backward of 65536 x 2047 against 2048), so the chunks start at the 16-byte boundaries of memory, the first before the row.  A thread's
+// rows are a multiple of 8 apart (the grid's size is, where it has more than one): the boundaries are the same in each.
+enum Mode { FULL, PLAIN, SHIFTED };
+
+// This thread's K chunks of a row.
+template <typename T, int TPR, int K, Mode MODE> struct Cols {
     static constexpr int V = Elem<T>::CH;
-    int lane, cols;
-    __device__ __forceinline__ Cols(int cols_) : lane((int)threadIdx.x % TPR), cols(cols_) {}
-    static constexpr bool whole(int k) { return FULL || k < K / 2; }
-    __device__ __forceinline__ int col(int k) const { return (k * TPR + lane) * V; }
+    int start, cols;             // start: the first chunk's column
+    __device__ __forceinline__ static int threads() { return TPR > 64 ? (int)blockDim.x : TPR; }
+    __device__ __forceinline__ Cols(int cols_, const T* first_row) : start((TPR > 64 ? (int)threadIdx.x : (int)threadIdx.x % TPR) * V), cols(cols_) {
+        if constexpr (MODE == SHIFTED) start -= (int)((uintptr_t)first_row / sizeof(T) % V);
+    }
+    static constexpr bool whole(int k) { return MODE == FULL || (MODE == PLAIN && k < K / 2); }
+    __device__ __forceinline__ static bool leads() { return TPR > 64 ? threadIdx.x == 0 : threadIdx.x % TPR == 0; }
+    __device__ __forceinline__ int col(int k) const { return k * threads() * V + start; }
     typedef Piece<T, int, TPR == 2> piece_t;             // (only rows of one or two chunks can have less than 16 bytes)
     __device__ __forceinline__ piece_t piece(int k) const { return piece_t(col(k), cols); }
     __device__ __forceinline__ bool own(int k, int e) const { return whole(k) || piece(k).own(e); }
@@ -159,26 +174,38 @@ template <typename T, int TPR, int K, bool FULL> struct Cols {
     }
 };
 
-template <typename T, int TPR, int K, bool FULL>
+template <typename T, int TPR, int K, Mode MODE>
 __global__ __launch_bounds__(block_threads(TPR)) void ln_fwd_kernel(const T* __restrict__ x, const float* __restrict__ w,
                                                                     const float* __restrict__ b, T* __restrict__ out, float* __restrict__ mean,
                                                                     float* __restrict__ rstd, int64_t rows, int cols, float eps, int relu) {
-    constexpr int V = Elem<T>::CH, R = block_threads(TPR) / TPR, WAVES = TPR / 64, LANES = wave_lanes(TPR);
+    constexpr int V = Elem<T>::CH, R = TPR > 64 ? 1 : 256 / TPR, LANES = wave_lanes(TPR);
+    constexpr bool WAVES = TPR > 64;                     // a row is several wavefronts'
     constexpr bool HOLD = holds_weights(TPR, K * V);
-    const Cols<T, TPR, K, FULL> at(cols);
+    const int64_t stride = (int64_t)gridDim.x * R;
+    int64_t row = (int64_t)blockIdx.x * R + (WAVES ? 0 : threadIdx.x / TPR);
+    const Cols<T, TPR, K, MODE> at(cols, x + row * cols);
     const float inv = 1.f / (float)cols;
-    __shared__ float2 part[2][WAVES > 1 ? WAVES : 1];    // mean and squares of each wavefront's columns, two rows' worth
-    __shared__ float counts[WAVES > 1 ? WAVES : 1];
+    __shared__ float2 part[2][WAVES ? 16 : 1];           // mean and squares of each wavefront's columns, two rows' worth
+    __shared__ float counts[WAVES ? 16 : 1];
+    if constexpr (WAVES) {
+        if (threadIdx.x < 16) {
+            part[0][threadIdx.x] = part[1][threadIdx.x] = make_float2(0.f, 0.f);
+            counts[threadIdx.x] = 0.f;
+        }
+        __syncthreads();
+    }
     float count = (float)(LANES * K * V);                 // elements of a row that this wavefront's (or group's) lanes own
-    if constexpr (!FULL) {
+    if constexpr (MODE != FULL) {
         count = 0.f;
 #pragma unroll
         for (int k = 0; k < K; ++k) count += (float)at.own(k);
         count = lanes_sum<LANES>(count);
-        if constexpr (WAVES > 1) {
-            if ((threadIdx.x & 63) == 0) counts[threadIdx.x >> 6] = count;
-            __syncthreads();
-        }
+    }
+    float wave_count = 0.f;                               // lane i of 16: wavefront i's
+    if constexpr (WAVES) {
+        if ((threadIdx.x & 63) == 0) counts[threadIdx.x >> 6] = count;
+        __syncthreads();
+        wave_count = counts[threadIdx.x & 15];
     }
     const float inv_count = count > 0.f ? 1.f / count : 0.f;
     float wf[HOLD ? K : 1][V], bf[HOLD ? K : 1][V];
@@ -189,8 +216,6 @@ __global__ __launch_bounds__(block_threads(TPR)) void ln_fwd_kernel(const T* __r
             at.load(b, 0.f, k, bf[k]);
         }
     }
-    const int64_t stride = (int64_t)gridDim.x * R;
-    int64_t row = (int64_t)blockIdx.x * R + threadIdx.x / TPR;
     uint4 q[K];
     if (row < rows) at.load(x + row * cols, q);
     for (int turn = 0; row < rows; row += stride, turn ^= 1) {      // (a workgroup with barriers has one row at a time: it leaves as one)
@@ -215,23 +240,13 @@ __global__ __launch_bounds__(block_threads(TPR)) void ln_fwd_kernel(const T* __r
                 ss = fmaf(d, d, ss);
             }
         ss = lanes_sum<LANES>(ss);
-        if constexpr (WAVES > 1) {       // the row's from the wavefronts': their squares about their own means, moved to the common one
+        if constexpr (WAVES) {           // the row's from the wavefronts': their squares about their own means, moved to the common one
             if ((threadIdx.x & 63) == 0) part[turn][threadIdx.x >> 6] = make_float2(m, ss);
             __syncthreads();             // (the other turn's slot is written only behind the next row's barrier: one barrier a row)
-            float2 p[WAVES];
-            m = 0.f;
-#pragma unroll
-            for (int i = 0; i < WAVES; ++i) {
-                p[i] = part[turn][i];
-                m = fmaf(p[i].x, FULL ? count : counts[i], m);
-            }
-            m = divide(m, (float)cols, inv);
-            ss = 0.f;
-#pragma unroll
-            for (int i = 0; i < WAVES; ++i) {
-                const float d = p[i].x - m;
-                ss += fmaf(d * d, FULL ? count : counts[i], p[i].y);
-            }
+            const float2 p = part[turn][threadIdx.x & 15];
+            m = divide(waves_sum(p.x * wave_count), (float)cols, inv);
+            const float d = p.x - m;
+            ss = waves_sum(wave_count > 0.f ? fmaf(d * d, wave_count, p.y) : 0.f);
         }
         const float r = rsqrtf(fmaf(ss, inv, eps));
 #pragma unroll
@@ -251,7 +266,7 @@ __global__ __launch_bounds__(block_threads(TPR)) void ln_fwd_kernel(const T* __r
             }
             at.store(out + row * cols, k, y);
         }
-        if (at.lane == 0) { mean[row] = m; rstd[row] = r; }
+        if (at.leads()) { mean[row] = m; rstd[row] = r; }
     }
 }
 
@@ -286,16 +301,16 @@ template <typename T, int K, bool ACT> struct RowData {
 };
 
 // the row's averages of g and g xhat from this thread's sums
-template <int TPR, int WAVES>
+template <int TPR>
 __device__ __forceinline__ void row_averages(float& c1, float& c2, float2* part, float inv) {
     c1 = lanes_sum<wave_lanes(TPR)>(c1);
     c2 = lanes_sum<wave_lanes(TPR)>(c2);
-    if constexpr (WAVES > 1) {
+    if constexpr (TPR > 64) {
         if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = make_float2(c1, c2);
         __syncthreads();
-        c1 = c2 = 0.f;
-#pragma unroll
-        for (int i = 0; i < WAVES; ++i) { c1 += part[i].x; c2 += part[i].y; }
+        const float2 p = part[threadIdx.x & 15];
+        c1 = waves_sum(p.x);
+        c2 = waves_sum(p.y);
     }
     c1 *= inv;
     c2 *= inv;
@@ -304,16 +319,22 @@ __device__ __forceinline__ void row_averages(float& c1, float& c2, float2* part,
 // dx, and this workgroup's sums for dweight and dbias.  A thread has the same columns in every row it works on: its parts of dweight and
 // dbias stay in registers until the last row.  Then the R row groups of a workgroup are added up in LDS and one partial row [2][cols] a
 // workgroup goes to scratch (partial == NULL: no weight, no sums).
-template <typename T, int TPR, int K, bool FULL, bool ACT>
+template <typename T, int TPR, int K, Mode MODE, bool ACT>
 __global__ __launch_bounds__(block_threads(TPR)) void ln_bwd_kernel(const T* __restrict__ x, const float* __restrict__ w,
                                                                     const float* __restrict__ mean, const float* __restrict__ rstd,
                                                                     const T* __restrict__ dout, const T* __restrict__ act, T* __restrict__ dx,
                                                                     float* __restrict__ partial, int64_t rows, int cols) {
-    constexpr int V = Elem<T>::CH, THREADS = block_threads(TPR), R = THREADS / TPR, WAVES = TPR / 64;
-    constexpr bool HOLD = holds_weights(TPR, K * V);
-    const Cols<T, TPR, K, FULL> at(cols);
+    constexpr int V = Elem<T>::CH, R = TPR > 64 ? 1 : 256 / TPR;
+    constexpr bool WAVES = TPR > 64, HOLD = holds_weights(TPR, K * V);
+    const int64_t stride = (int64_t)gridDim.x * R;
+    int64_t row = (int64_t)blockIdx.x * R + (WAVES ? 0 : threadIdx.x / TPR);
+    const Cols<T, TPR, K, MODE> at(cols, x + row * cols);
     const float inv = 1.f / (float)cols;
-    __shared__ float2 part[2][WAVES > 1 ? WAVES : 1];
+    __shared__ float2 part[2][WAVES ? 16 : 1];
+    if constexpr (WAVES) {
+        if (threadIdx.x < 16) part[0][threadIdx.x] = part[1][threadIdx.x] = make_float2(0.f, 0.f);
+        __syncthreads();
+    }
     float wf[HOLD ? K : 1][V], dw[K][V], db[K][V];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
@@ -321,8 +342,6 @@ __global__ __launch_bounds__(block_threads(TPR)) void ln_bwd_kernel(const T* __r
 #pragma unroll
         for (int e = 0; e < V; ++e) dw[k][e] = db[k][e] = 0.f;
     }
-    const int64_t stride = (int64_t)gridDim.x * R;
-    int64_t row = (int64_t)blockIdx.x * R + threadIdx.x / TPR;
     RowData<T, K, ACT> in;
     if (row < rows) in.load(at, x, dout, act, mean, rstd, row, cols);
     for (int turn = 0; row < rows; row += stride, turn ^= 1) {
@@ -349,7 +368,7 @@ __global__ __launch_bounds__(block_threads(TPR)) void ln_bwd_kernel(const T* __r
                 c2 = fmaf(go, xh[k][e], c2);
             }
         }
-        row_averages<TPR, WAVES>(c1, c2, part[turn], inv);
+        row_averages<TPR>(c1, c2, part[turn], inv);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             float y[V];
@@ -373,7 +392,7 @@ __global__ __launch_bounds__(block_threads(TPR)) void ln_bwd_kernel(const T* __r
                 for (int e = 0; e < V; ++e)
                     if (at.own(k, e)) red[threadIdx.x / TPR * (TPR * K * V) + at.first_col(k) + e] = v[k][e];
             __syncthreads();
-            for (int c = threadIdx.x; c < cols; c += THREADS) {
+            for (int c = threadIdx.x; c < cols; c += 256) {
                 float s = 0.f;
 #pragma unroll 8
                 for (int i = 0; i < R; ++i) s += red[i * (TPR * K * V) + c];
@@ -399,12 +418,18 @@ __global__ __launch_bounds__(block_threads(TPR)) void ln_bwd_few_kernel(const T*
                                                                         T* __restrict__ dx, float* __restrict__ dw_out,
                                                                         float* __restrict__ db_out, int accumulate, int rows, int cols,
                                                                         int dx_blocks) {
-    constexpr int V = Elem<T>::CH, THREADS = block_threads(TPR), R = THREADS / TPR, WAVES = TPR / 64;
+    constexpr int V = Elem<T>::CH, R = TPR > 64 ? 1 : 256 / TPR;
+    constexpr bool WAVES = TPR > 64;
+    const int waves = (int)blockDim.x / 64;
     if ((int)blockIdx.x < dx_blocks) {
-        const Cols<T, TPR, K, false> at(cols);
-        __shared__ float2 part[WAVES > 1 ? WAVES : 1];
-        const int row = (int)blockIdx.x * R + (int)threadIdx.x / TPR;
-        if (row >= rows) return;                            // (with barriers a workgroup has one row: it leaves as one)
+        const Cols<T, TPR, K, PLAIN> at(cols, x);
+        __shared__ float2 part[WAVES ? 16 : 1];
+        if constexpr (WAVES) {
+            if (threadIdx.x < 16) part[threadIdx.x] = make_float2(0.f, 0.f);
+            __syncthreads();
+        }
+        const int row = (int)blockIdx.x * R + (WAVES ? 0 : (int)threadIdx.x / TPR);
+        if (row >= rows) return;                            // (with barriers a workgroup has one row, and there are no more of them)
         RowData<T, K, ACT> in;
         in.load(at, x, dout, act, mean, rstd, row, cols);
         float xh[K][V], g[K][V], c1 = 0.f, c2 = 0.f;
@@ -422,7 +447,7 @@ __global__ __launch_bounds__(block_threads(TPR)) void ln_bwd_few_kernel(const T*
                 c2 = fmaf(go, xh[k][e], c2);
             }
         }
-        row_averages<TPR, WAVES>(c1, c2, part, 1.f / (float)cols);
+        row_averages<TPR>(c1, c2, part, 1.f / (float)cols);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             float y[V];
@@ -432,15 +457,16 @@ __global__ __launch_bounds__(block_threads(TPR)) void ln_bwd_few_kernel(const T*
         }
         return;
     }
-    constexpr int LANES = 8, ROWS = THREADS / LANES;
-    __shared__ float red[2][THREADS / 64][LANES * V];
+    constexpr int LANES = 8;
+    const int step = (int)blockDim.x / LANES;
+    __shared__ float red[2][block_threads(TPR) / 64][LANES * V];
     const int lane = (int)threadIdx.x % LANES;
     const Piece<T, int, TPR == 2> piece((((int)blockIdx.x - dx_blocks) * LANES + lane) * V, cols);
     float dw[V], db[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) dw[e] = db[e] = 0.f;
 #pragma unroll 4
-    for (int row = (int)threadIdx.x / LANES; row < rows; row += ROWS) {
+    for (int row = (int)threadIdx.x / LANES; row < rows; row += step) {
         const int64_t i = (int64_t)row * cols;
         float xv[V], d[V];
         Chunk<T>::unpack(piece.load(x + i), xv);
@@ -471,8 +497,7 @@ __global__ __launch_bounds__(block_threads(TPR)) void ln_bwd_few_kernel(const T*
 #pragma unroll
         for (int e = 0; e < V; ++e) {
             float sw = 0.f, sb = 0.f;
-#pragma unroll
-            for (int i = 0; i < THREADS / 64; ++i) { sw += red[0][i][lane * V + e]; sb += red[1][i][lane * V + e]; }
+            for (int i = 0; i < waves; ++i) { sw += red[0][i][lane * V + e]; sb += red[1][i][lane * V + e]; }
             if (piece.own(e)) {
                 const int c = piece.from + e;
                 dw_out[c] = accumulate ? dw_out[c] + sw : sw;
@@ -652,74 +677,95 @@ __global__ __launch_bounds__(256) void ln_bwd_long_dw_kernel(const T* __restrict
 
 // ---- which split -----------------------------------------------------------------------------------------------------------------------
 // Threads a row and chunks a thread, from the row's number of 16-byte chunks.  Up to 64 chunks: one a lane, the smallest power of two of
-// lanes (several rows share a wavefront).  Then a wavefront with up to KMAX a lane, then a workgroup of 256 .. 1024.  KMAX: what the
-// registers hold with four wavefronts a SIMD -- 4 forward; backward, which keeps a weight and two sums a column, 16 values (4 fp32
-// chunks, 2 bf16).  At 512 threads fp32 stops at 2: 16384 x 8192 takes 195 / 289 us forward / backward as 1024 threads of 2 chunks, 200 /
-// 309 as 512 of 4 (bf16, 8192 x 16384 forward: 107 against 99, the other way).
-struct Split { int tpr, k; };
+// lanes (several rows share a wavefront).  Then a wavefront with up to KMAX a lane, then a workgroup of the wavefronts it takes, up to 16.
+// KMAX: what the registers hold with four wavefronts a SIMD -- 4 forward; backward, which keeps a weight and two sums a column, 16 values
+// (4 fp32 chunks, 2 bf16).  From 5 wavefronts on fp32 stops at 2: 16384 x 8192 takes 195 / 289 us forward / backward as 1024 threads of 2
+// chunks, 200 / 309 as 512 of 4 (bf16, 8192 x 16384 forward: 107 against 99, the other way).
+struct Split { int tpr, k, threads; int64_t chunks; bool shifted = false; };      // tpr, k: the kernel's; threads: a workgroup's
 Split ln_split(int dtype, int64_t chunks, int kmax) {
     if (chunks <= 64) {
         int tpr = 2;
         while (tpr < chunks) tpr *= 2;
-        return {tpr, 1};
+        return {tpr, 1, 256, chunks};
     }
     for (int tpr = 64; tpr <= 1024; tpr = tpr == 64 ? 256 : tpr * 2)
         for (int k = 1; k <= (dtype == VINCE_F32 && tpr == 512 ? 2 : kmax); k *= 2)
-            if ((int64_t)tpr * k >= chunks) return {tpr, k};
-    return {0, 0};
+            if ((int64_t)tpr * k >= chunks) return {tpr, k, tpr == 64 ? 256 : (int)((chunks + 64 * k - 1) / (64 * k)) * 64, chunks};
+    return {0, 0, 0, chunks};
 }
-int ln_chunks(int dtype, int cols) { const int v = dtype == VINCE_F32 ? 4 : 8; return (cols + v - 1) / v; }
-constexpr int LN_FWD_K = 4;
-constexpr int ln_bwd_k(int dtype) { return dtype == VINCE_F32 ? 4 : 2; }
+int64_t ln_chunks(int dtype, int64_t cols) { const int v = dtype == VINCE_F32 ? 4 : 8; return (cols + v - 1) / v; }
+int ln_bwd_k(int dtype) { return dtype == VINCE_F32 ? 4 : 2; }
+Split ln_plain_split(int dtype, int cols, int kmax) { return ln_split(dtype, ln_chunks(dtype, cols), kmax); }
+Split ln_row_split(int dtype, int cols, int kmax) {
+    if (dtype == VINCE_BF16 && (cols & 1) && cols >= 16) {      // (shorter rows have hardly a whole chunk to align)
+        Split s = ln_split(dtype, ln_chunks(dtype, cols + (int64_t)7), kmax);
+        s.shifted = true;
+        if (s.tpr) return s;
+    }
+    return ln_plain_split(dtype, cols, kmax);
+}
+Split ln_fwd_split(int dtype, int cols) { return ln_row_split(dtype, cols, 4); }
+Split ln_bwd_split(int dtype, int cols) { return ln_row_split(dtype, cols, ln_bwd_k(dtype)); }
+Split ln_few_split(int dtype, int cols) { return ln_plain_split(dtype, cols, ln_bwd_k(dtype)); }
 
 // Workgroups: as many as have 4 MB of rows in their registers -- 2^18 chunks, of one tensor forward, of two backward -- and one a CU at
 // least; each goes through its share of the rows.  More rows at a time are slower, fewer too (forward, 65536 x 2048 bf16, us at 256 / 512
 // / 1024 / 2048 workgroups of 4 chunks a thread: 91 / 98 / 99 / 97; 10^6 x 128, of 1: 188 / 113 / 88 / 104; backward, 32768 x 4096, of 2:
-// 144 / 150 / 172 at 256 / 512 / 1024, where every workgroup also leaves a partial row of 8 bytes a column to be read again).
+// 144 / 150 / 172 at 256 / 512 / 1024, where every workgroup also leaves a partial row of 8 bytes a column to be read again).  The same
+// number for every CU: 60000 x 1000 bf16 takes 44 us with 512, 50 with 520.  (Any multiple of 8 would do for Mode.)
 int64_t ln_blocks(const Split& s, int64_t in_flight) {
-    const int64_t n = s.tpr ? in_flight / (block_threads(s.tpr) * s.k) : 1024;
-    return n < 256 ? 256 : n;
+    const int64_t n = s.tpr ? in_flight / ((s.tpr > 64 ? 1 : 256 / s.tpr) * s.chunks) : 1024;
+    return n < 384 ? 256 : (n + 128) / 256 * 256;
 }
 int64_t ln_fwd_blocks(int64_t rows, const Split& s) {
-    const int64_t r = s.tpr ? block_threads(s.tpr) / s.tpr : 1, want = (rows + r - 1) / r, most = ln_blocks(s, 1 << 18);
+    const int64_t r = s.tpr && s.tpr <= 64 ? 256 / s.tpr : 1, want = (rows + r - 1) / r, most = ln_blocks(s, 1 << 18);
     return want < most ? want : most;
 }
 // (at least four rows for each row group, so that the partial rows stay a small part of what is read)
 int ln_bwd_blocks(int64_t rows, const Split& s) {
-    const int64_t per = s.tpr ? 4 * (block_threads(s.tpr) / s.tpr) : 4, most = ln_blocks(s, 1 << 17);
-    const int64_t n = (rows + per - 1) / per;
-    return (int)(n < 1 ? 1 : n > most ? most : n);
+    const int64_t per = s.tpr && s.tpr <= 64 ? 4 * (256 / s.tpr) : 4, most = ln_blocks(s, 1 << 17);
+    const int64_t n = ((rows + per - 1) / per + 7) / 8 * 8;
+    return (int)(n > most ? most : n);
 }
 // Few rows (ln_bwd_few_kernel): one launch for two and no scratch, against reading x and dout twice and column sums that one workgroup makes
 // over all rows.  us of a call, two launches / one: 256 x 2048 fp32 8.4 / 5.3, 512 x 8192 bf16 14.7 / 9.9, 1024 x 512 fp32 8.1 / 5.7, 1024 x
 // 2048 bf16 9.0 / 10.0 (and 2 us for the scratch's allocation).
-bool ln_bwd_few(int dtype, int64_t rows, int cols, const Split& s) {
-    return s.tpr && rows <= 1024 && rows * ln_chunks(dtype, cols) <= (rows <= 512 ? 1 << 19 : 1 << 18);
+bool ln_bwd_few(int dtype, int64_t rows, int cols) {
+    return ln_few_split(dtype, cols).tpr && rows <= 1024 && rows * ln_chunks(dtype, cols) <= (rows <= 512 ? 1 << 19 : 1 << 18);
 }
 
 template <typename T, int TPR, int K>
-void launch_fwd(const void* x, const float* w, const float* b, void* out, float* mean, float* rstd, int64_t rows, int cols, float eps, int relu,
-                hipStream_t st) {
-    constexpr int THREADS = block_threads(TPR);
-    const dim3 grid((unsigned)ln_fwd_blocks(rows, {TPR, K}));
-    if (cols == TPR * K * Elem<T>::CH)
-        hipLaunchKernelGGL((ln_fwd_kernel<T, TPR, K, true>), grid, dim3(THREADS), 0, st, (const T*)x, w, b, (T*)out, mean, rstd, rows, cols, eps, relu);
-    else
-        hipLaunchKernelGGL((ln_fwd_kernel<T, TPR, K, false>), grid, dim3(THREADS), 0, st, (const T*)x, w, b, (T*)out, mean, rstd, rows, cols, eps, relu);
+void launch_fwd(bool shifted, const dim3& grid, const dim3& block, const void* x, const float* w, const float* b, void* out, float* mean, float* rstd, int64_t rows, int cols,
+                float eps, int relu, hipStream_t st) {
+#define LN_LAUNCH(MODE) \
+    hipLaunchKernelGGL((ln_fwd_kernel<T, TPR, K, MODE>), grid, block, 0, st, (const T*)x, w, b, (T*)out, mean, rstd, rows, cols, eps, relu)
+    if (cols == (TPR > 64 ? (int)block.x : TPR) * K * Elem<T>::CH) {
+        LN_LAUNCH(FULL);
+        return;
+    }
+    if constexpr (sizeof(T) == 2) {
+        if (shifted) {
+            LN_LAUNCH(SHIFTED);
+            return;
+        }
+    }
+    LN_LAUNCH(PLAIN);
+#undef LN_LAUNCH
 }
 
 template <typename T>
 void run_fwd(int dtype, const void* x, const float* w, const float* b, void* out, float* mean, float* rstd, int64_t rows, int cols, float eps,
              int relu, hipStream_t st) {
-    const Split s = ln_split(dtype, ln_chunks(dtype, cols), LN_FWD_K);
+    const Split s = ln_fwd_split(dtype, cols);
+    const dim3 grid((unsigned)ln_fwd_blocks(rows, s)), block((unsigned)s.threads);
 #define LN_CASE(TPR, K) \
-    if (s.tpr == TPR && s.k == K) return launch_fwd<T, TPR, K>(x, w, b, out, mean, rstd, rows, cols, eps, relu, st)
+    if (s.tpr == TPR && s.k == K) return launch_fwd<T, TPR, K>(s.shifted, grid, block, x, w, b, out, mean, rstd, rows, cols, eps, relu, st)
     LN_CASE(2, 1); LN_CASE(4, 1); LN_CASE(8, 1); LN_CASE(16, 1); LN_CASE(32, 1); LN_CASE(64, 1); LN_CASE(64, 2); LN_CASE(64, 4);
     LN_CASE(256, 2); LN_CASE(256, 4); LN_CASE(1024, 4);
     if constexpr (sizeof(T) == 4) { LN_CASE(1024, 2); }
     else { LN_CASE(512, 4); }
 #undef LN_CASE
-    hipLaunchKernelGGL(ln_fwd_long_kernel<T>, dim3((unsigned)ln_fwd_blocks(rows, s)), dim3(1024), 0, st, (const T*)x, w, b, (T*)out, mean, rstd,
+    hipLaunchKernelGGL(ln_fwd_long_kernel<T>, grid, dim3(1024), 0, st, (const T*)x, w, b, (T*)out, mean, rstd,
                        rows, cols, eps, relu);
 }
 
@@ -730,31 +776,39 @@ struct BwdArgs {
     float *dw, *db, *partial;      // partial == NULL with dw: few rows, one launch
     int accumulate;
     int64_t rows;
-    int cols, blocks;
+    int cols, blocks, threads;     // blocks, threads: the launch's
+    bool shifted;
 };
 
 template <typename T, int TPR, int K> void launch_bwd(const BwdArgs& a, hipStream_t st) {
-    constexpr int THREADS = block_threads(TPR), R = THREADS / TPR, V = Elem<T>::CH;
+    constexpr int R = TPR > 64 ? 1 : 256 / TPR, V = Elem<T>::CH;
     if (a.dw && !a.partial) {
         const int dx_blocks = (int)((a.rows + R - 1) / R), dw_blocks = (a.cols + 8 * V - 1) / (8 * V);
 #define LN_LAUNCH(ACT)                                                                                                                        \
-    if ((a.act != nullptr) == ACT)                                                                                                            \
-    hipLaunchKernelGGL((ln_bwd_few_kernel<T, TPR, K, ACT>), dim3(dx_blocks + dw_blocks), dim3(THREADS), 0, st, (const T*)a.x, a.w, a.mean, a.rstd, \
+    hipLaunchKernelGGL((ln_bwd_few_kernel<T, TPR, K, ACT>), dim3(dx_blocks + dw_blocks), dim3(a.threads), 0, st, (const T*)a.x, a.w, a.mean, a.rstd, \
                        (const T*)a.dout, (const T*)a.act, (T*)a.dx, a.dw, a.db, a.accumulate, (int)a.rows, a.cols, dx_blocks)
-        LN_LAUNCH(false);
-        LN_LAUNCH(true);
+        if (a.act) LN_LAUNCH(true);
+        else LN_LAUNCH(false);
 #undef LN_LAUNCH
         return;
     }
-    const bool full = a.cols == TPR * K * V;
-#define LN_LAUNCH(FULL, ACT)                                                                                                               \
-    if (full == FULL && (a.act != nullptr) == ACT)                                                                                         \
-    hipLaunchKernelGGL((ln_bwd_kernel<T, TPR, K, FULL, ACT>), dim3(a.blocks), dim3(THREADS), 0, st, (const T*)a.x, a.w, a.mean, a.rstd,    \
+#define LN_LAUNCH(MODE, ACT)                                                                                                               \
+    hipLaunchKernelGGL((ln_bwd_kernel<T, TPR, K, MODE, ACT>), dim3(a.blocks), dim3(a.threads), 0, st, (const T*)a.x, a.w, a.mean, a.rstd,  \
                        (const T*)a.dout, (const T*)a.act, (T*)a.dx, a.partial, a.rows, a.cols)
-    LN_LAUNCH(true, false);
-    LN_LAUNCH(true, true);
-    LN_LAUNCH(false, false);
-    LN_LAUNCH(false, true);
+    if (a.cols == (TPR > 64 ? a.threads : TPR) * K * V) {
+        if (a.act) LN_LAUNCH(FULL, true);
+        else LN_LAUNCH(FULL, false);
+        return;
+    }
+    if constexpr (sizeof(T) == 2) {
+        if (a.shifted) {
+            if (a.act) LN_LAUNCH(SHIFTED, true);
+            else LN_LAUNCH(SHIFTED, false);
+            return;
+        }
+    }
+    if (a.act) LN_LAUNCH(PLAIN, true);
+    else LN_LAUNCH(PLAIN, false);
 #undef LN_LAUNCH
 }
 
@@ -795,8 +849,7 @@ extern "C" int vince_layer_norm_fwd(int dtype, const void* x, const float* weigh
 
 extern "C" size_t vince_layer_norm_bwd_scratch_bytes(int dtype, int64_t rows, int32_t cols) {
     if (rows <= 0 || cols <= 0) return 0;
-    const Split s = ln_split(dtype, ln_chunks(dtype, cols), ln_bwd_k(dtype));
-    return ln_bwd_few(dtype, rows, cols, s) ? 0 : (size_t)ln_bwd_blocks(rows, s) * 2 * (size_t)cols * sizeof(float);
+    return ln_bwd_few(dtype, rows, cols) ? 0 : (size_t)ln_bwd_blocks(rows, ln_bwd_split(dtype, cols)) * 2 * (size_t)cols * sizeof(float);
 }
 
 extern "C" int vince_layer_norm_bwd(int dtype, const void* x, const float* weight, const float* mean, const float* rstd, const void* dout,
@@ -805,14 +858,14 @@ extern "C" int vince_layer_norm_bwd(int dtype, const void* x, const float* weigh
     LN_CHECK("vince_layer_norm_bwd");
     VINCE_CHECK_ARG((dweight == nullptr) == (dbias == nullptr), VINCE_E_ARG, "vince_layer_norm_bwd: dweight and dbias come together");
     hipStream_t st = (hipStream_t)stream;
-    const Split s = ln_split(dtype, ln_chunks(dtype, cols), ln_bwd_k(dtype));
+    const bool few = rows > 0 && dweight && ln_bwd_few(dtype, rows, cols);
+    const Split s = few ? ln_few_split(dtype, cols) : ln_bwd_split(dtype, cols);
     const int blocks = ln_bwd_blocks(rows, s);
-    const bool few = rows > 0 && ln_bwd_few(dtype, rows, cols, s);
     if (rows > 0) {
         VINCE_CHECK_ARG(x && mean && rstd && dout && dx, VINCE_E_ARG, "vince_layer_norm_bwd: null pointer");
         const size_t need = dweight ? vince_layer_norm_bwd_scratch_bytes(dtype, rows, cols) : 0;
         VINCE_CHECK_ARG(need == 0 || (scratch && scratch_bytes >= need), VINCE_E_ARG, "vince_layer_norm_bwd: scratch of %zu bytes", scratch_bytes);
-        const BwdArgs a = {x, dout, act, weight, mean, rstd, dx, dweight, dbias, few || !dweight ? nullptr : (float*)scratch, accumulate, rows, cols, blocks};
+        const BwdArgs a = {x, dout, act, weight, mean, rstd, dx, dweight, dbias, few || !dweight ? nullptr : (float*)scratch, accumulate, rows, cols, blocks, s.threads, s.shifted};
         if (dtype == VINCE_F32) run_bwd<float>(s, a, st);
         else run_bwd<bf16_t>(s, a, st);
         VINCE_CHECK_LAUNCH();
