@@ -544,7 +544,7 @@ int vince_colsum(const float* x, float* out, int32_t rows, int32_t cols, void* s
  *     dweight = sum over the rows of d xhat, dbias = sum of d (accumulate != 0: added to what is there), fixed order of summation.
  *     dweight and dbias may both be NULL.  scratch: vince_layer_norm_bwd_scratch_bytes(), not read before it is written.
  * No alignment beyond the element's is needed, rows may be 0 (cols >= 1), a value that is not finite spoils its own row (and its
- * columns' sums) only.  (ABI 13) */
+ * columns' sums) only.  No output may share memory with an input or another output.  (ABI 13) */
 int vince_layer_norm_fwd(int dtype, const void* x, const float* weight, const float* bias, void* out, float* mean, float* rstd,
                          int64_t rows, int32_t cols, float eps, int32_t relu, void* stream);
 size_t vince_layer_norm_bwd_scratch_bytes(int dtype, int64_t rows, int32_t cols);

@@ -45,7 +45,7 @@ def build(force=False, verbose=True, measure=False):
     os.makedirs(LIBDIR, exist_ok=True)
     os.makedirs(OBJDIR, exist_ok=True)
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-    headers = [os.path.join(CSRC, "common.h"), os.path.join(CSRC, "conv_core.h"), os.path.join(CSRC, "conv_igemm_impl.h"), os.path.join(CSRC, "conv_wgrad.h"), os.path.join(os.path.dirname(HERE), "include", "vince_hip.h")]
+    headers = [os.path.abspath(__file__), os.path.join(CSRC, "common.h"), os.path.join(CSRC, "conv_core.h"), os.path.join(CSRC, "conv_igemm_impl.h"), os.path.join(CSRC, "conv_wgrad.h"), os.path.join(os.path.dirname(HERE), "include", "vince_hip.h")]
     jobs = []
     objs = []
     for s in SOURCES:

@@ -723,7 +723,7 @@ int64_t ln_fwd_blocks(int64_t rows, const Split& s) {
 }
 // (at least four rows for each row group, so that the partial rows stay a small part of what is read)
 int ln_bwd_blocks(int64_t rows, const Split& s) {
-    const int64_t per = s.tpr && s.tpr <= 64 ? 4 * (256 / s.tpr) : 4, most = ln_blocks(s, 1 << 17);
+    const int64_t per = s.tpr && s.tpr <= 64 ? 4 * (256 / s.tpr) : 4, most = s.tpr ? ln_blocks(s, 1 << 17) : 256;
     const int64_t n = ((rows + per - 1) / per + 7) / 8 * 8;
     return (int)(n > most ? most : n);
 }
