@@ -43,12 +43,13 @@ def test_layer_norm_refusals(L):
 
 
 def test_grad_entry_point_refusals(L):
-    norm = lambda **k: L.vince_grad_norm(*[{**dict(table=PTR, chunks=3, limit=1.0, clip=PTR, scratch=PTR, nbytes=1 << 20, stream=NULL), **k}[n]  # noqa: E731
+    norm = lambda **k: L.vince_grad_norm(*[{**dict(table=PTR, chunks=300, limit=1.0, clip=PTR, scratch=PTR, nbytes=1 << 20, stream=NULL), **k}[n]  # noqa: E731
                                            for n in ("table", "chunks", "limit", "clip", "scratch", "nbytes", "stream")])
     assert norm(table=NULL) == norm(clip=NULL) == norm(scratch=NULL) == norm(chunks=-1) == -5
     assert norm(limit=-1.0) == -5 and norm(limit=float("nan")) == -5 and b"max_norm" in L.vince_last_error()
     assert norm(nbytes=0) == -5 and b"scratch" in L.vince_last_error()
-    assert L.vince_grad_clip(PTR, 3, -1.0, PTR, PTR, 1 << 20, NULL) == -5
+    assert norm(chunks=3, table=NULL) == norm(chunks=3, clip=NULL) == norm(chunks=3, limit=-1.0) == -5
+    assert L.vince_grad_clip(PTR, 300, -1.0, PTR, PTR, 1 << 20, NULL) == L.vince_grad_clip(PTR, 3, -1.0, PTR, PTR, 1 << 20, NULL) == -5
     assert L.vince_grad_scale(NULL, 3, PTR, NULL) == -5 and L.vince_grad_scale(PTR, 3, NULL, NULL) == -5
     assert L.vince_grad_scale(NULL, 0, PTR, NULL) == 0
     sgd = lambda **k: L.vince_sgd_flat_clip(*[{**dict(p=PTR, g=PTR, b=PTR, n=16, lr=0.1, mom=0.9, wd=0.0, gs=1.0, clip=PTR, stream=NULL), **k}[n]  # noqa: E731

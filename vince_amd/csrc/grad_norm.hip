@@ -12,6 +12,7 @@ constexpr int GRAD_CHUNK_MIN = 2048, GRAD_CHUNK_MAX = 16384;
 // streams.  us at 256 / 512 / 1024 / 2048 of them, 160 M fp32: norm 126 / 103 / 107 / 112 (6.2 TB/s at 512), scaling 219 / 244 / 246 / 247;
 // norm and SGD step of 28 M at 256 / 512: 120 / 112.  (A piece's entry is read when the piece begins: read ahead, scaling takes 247 us at
 // 256, the norm 107 at 512.)
+constexpr int SMALL_CHUNKS = 64;
 constexpr int GRAD_NORM_BLOCKS = 512, GRAD_SCALE_BLOCKS = 256, SGD_BLOCKS = 512;
 constexpr uint32_t GRAD_BF16 = 1u << 31;
 
@@ -50,10 +51,11 @@ __device__ __forceinline__ void store16(void* p, const uint4& v) {
     *(global_u32x4_any_t*)p = w;
 }
 
-template <typename T> __device__ __forceinline__ double squares_of(const T* __restrict__ g, int n) {
-    constexpr int V = Elem<T>::CH, STEP = 256 * V, DEEP = 4;
+// this thread's share of a piece's sum of squares; THREADS of them, `thread` the number of this one
+template <int THREADS, typename T> __device__ __forceinline__ double squares_of(const T* __restrict__ g, int n, int thread) {
+    constexpr int V = Elem<T>::CH, STEP = THREADS * V, DEEP = 4;
     double s0 = 0.0, s1 = 0.0;
-    int i = threadIdx.x * V;
+    int i = thread * V;
     for (; i + (DEEP - 1) * STEP + V <= n; i += DEEP * STEP) {       // DEEP loads are in flight before the first is used
         uint4 q[DEEP];
 #pragma unroll
@@ -90,7 +92,7 @@ __global__ __launch_bounds__(256) void grad_squares_kernel(const GradChunk* __re
     for (int64_t c = blockIdx.x; c < chunks; c += gridDim.x) {
         const GradChunk k = table[c];
         const int n = (int)(k.n & ~GRAD_BF16);
-        const double s = k.n & GRAD_BF16 ? squares_of((const bf16_t*)k.data, n) : squares_of((const float*)k.data, n);
+        const double s = k.n & GRAD_BF16 ? squares_of<256>((const bf16_t*)k.data, n, threadIdx.x) : squares_of<256>((const float*)k.data, n, threadIdx.x);
         sum = fma((double)k.scale * (double)k.scale, s, sum);
     }
     sum = block_sum(sum);
@@ -99,11 +101,14 @@ __global__ __launch_bounds__(256) void grad_squares_kernel(const GradChunk* __re
 
 // [norm, coefficient] from the workgroups' sums, by every thread of a workgroup of 256: norm = sqrt(sum), coefficient =
 // min(1, max_norm / (norm + 1e-6)); an infinite max_norm clips nothing, a NaN norm gives a NaN coefficient
+__device__ __forceinline__ float2 clip_of(double sum, float max_norm) {
+    const double norm = sqrt(sum), c = (double)max_norm / (norm + 1e-6);
+    return make_float2((float)norm, max_norm == INFINITY || c > 1.0 ? 1.f : (float)c);
+}
 __device__ __forceinline__ float2 clip_of(const double* __restrict__ partial, int n, float max_norm) {
     double s = 0.0;
     for (int i = threadIdx.x; i < n; i += 256) s += partial[i];
-    const double norm = sqrt(block_sum(s)), c = (double)max_norm / (norm + 1e-6);
-    return make_float2((float)norm, max_norm == INFINITY || c > 1.0 ? 1.f : (float)c);
+    return clip_of(block_sum(s), max_norm);
 }
 
 __global__ __launch_bounds__(256) void grad_clip_kernel(const double* __restrict__ partial, int n, float max_norm, float* __restrict__ clip) {
@@ -111,9 +116,9 @@ __global__ __launch_bounds__(256) void grad_clip_kernel(const double* __restrict
     if (threadIdx.x == 0) { clip[0] = r.x; clip[1] = r.y; }
 }
 
-template <typename T> __device__ __forceinline__ void scale_piece(T* __restrict__ g, int n, float f) {
-    constexpr int V = Elem<T>::CH, STEP = 256 * V, DEEP = 4;
-    int i = threadIdx.x * V;
+template <int THREADS, typename T> __device__ __forceinline__ void scale_piece(T* __restrict__ g, int n, float f, int thread) {
+    constexpr int V = Elem<T>::CH, STEP = THREADS * V, DEEP = 4;
+    int i = thread * V;
     for (; i + (DEEP - 1) * STEP + V <= n; i += DEEP * STEP) {
         uint4 q[DEEP];
 #pragma unroll
@@ -157,8 +162,40 @@ __global__ __launch_bounds__(256) void grad_scale_kernel(const GradChunk* __rest
     for (int64_t c = blockIdx.x; c < chunks; c += gridDim.x) {
         const GradChunk k = table[c];
         const int n = (int)(k.n & ~GRAD_BF16);
-        if (k.n & GRAD_BF16) scale_piece((bf16_t*)k.data, n, f);
-        else scale_piece((float*)k.data, n, f);
+        if (k.n & GRAD_BF16) scale_piece<256>((bf16_t*)k.data, n, f, threadIdx.x);
+        else scale_piece<256>((float*)k.data, n, f, threadIdx.x);
+    }
+}
+
+// Few pieces (SMALL_CHUNKS): everything in one workgroup, a piece to a wavefront, and in one launch without scratch.
+template <bool SCALE>
+__global__ __launch_bounds__(1024) void grad_small_kernel(const GradChunk* __restrict__ table, int chunks, float max_norm, float* __restrict__ clip) {
+    __shared__ double red[16];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    double sum = 0.0;
+    for (int c = wave; c < chunks; c += 16) {
+        const GradChunk k = table[c];
+        const int n = (int)(k.n & ~GRAD_BF16);
+        const double s = k.n & GRAD_BF16 ? squares_of<64>((const bf16_t*)k.data, n, lane) : squares_of<64>((const float*)k.data, n, lane);
+        sum = fma((double)k.scale * (double)k.scale, s, sum);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+    if (lane == 0) red[wave] = sum;
+    __syncthreads();
+    sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sum += red[i];
+    const float2 r = clip_of(sum, max_norm);
+    if (threadIdx.x == 0) { clip[0] = r.x; clip[1] = r.y; }
+    if constexpr (SCALE) {
+        if (r.y == 1.f) return;
+        for (int c = wave; c < chunks; c += 16) {        // (the pieces that this wavefront itself has read)
+            const GradChunk k = table[c];
+            const int n = (int)(k.n & ~GRAD_BF16);
+            if (k.n & GRAD_BF16) scale_piece<64>((bf16_t*)k.data, n, r.y, lane);
+            else scale_piece<64>((float*)k.data, n, r.y, lane);
+        }
     }
 }
 
@@ -238,18 +275,24 @@ extern "C" int vince_grad_table_fill(const vince_grad_tensor* tensors, int32_t c
     return VINCE_OK;
 }
 
-extern "C" size_t vince_grad_norm_scratch_bytes(int64_t chunks) { return chunks > 0 ? (size_t)blocks_of(chunks, GRAD_NORM_BLOCKS) * sizeof(double) : 0; }
+extern "C" size_t vince_grad_norm_scratch_bytes(int64_t chunks) {
+    return chunks > SMALL_CHUNKS ? (size_t)blocks_of(chunks, GRAD_NORM_BLOCKS) * sizeof(double) : 0;
+}
 
 #define GRAD_NORM_CHECK(name)                                                                                                              \
-    VINCE_CHECK_ARG(chunks >= 0 && clip && (chunks == 0 || (table && scratch)), VINCE_E_ARG, name ": bad arguments");                      \
+    VINCE_CHECK_ARG(chunks >= 0 && clip && (chunks == 0 || table) && (chunks <= SMALL_CHUNKS || scratch), VINCE_E_ARG, name ": bad arguments"); \
     VINCE_CHECK_ARG(max_norm >= 0.f, VINCE_E_ARG, name ": max_norm=%g", (double)max_norm);                                                 \
     VINCE_CHECK_ARG(scratch_bytes >= vince_grad_norm_scratch_bytes(chunks), VINCE_E_ARG, name ": scratch of %zu bytes", scratch_bytes)
 
 extern "C" int vince_grad_norm(const void* table, int64_t chunks, float max_norm, float* clip, void* scratch, size_t scratch_bytes, void* stream) {
     GRAD_NORM_CHECK("vince_grad_norm");
+    if (chunks <= SMALL_CHUNKS) {
+        hipLaunchKernelGGL(grad_small_kernel<false>, dim3(1), dim3(1024), 0, (hipStream_t)stream, (const GradChunk*)table, (int)chunks, max_norm, clip);
+        VINCE_CHECK_LAUNCH();
+        return VINCE_OK;
+    }
     const int blocks = blocks_of(chunks, GRAD_NORM_BLOCKS);
-    if (blocks > 0)
-        hipLaunchKernelGGL(grad_squares_kernel, dim3(blocks), dim3(256), 0, (hipStream_t)stream, (const GradChunk*)table, chunks, (double*)scratch);
+    hipLaunchKernelGGL(grad_squares_kernel, dim3(blocks), dim3(256), 0, (hipStream_t)stream, (const GradChunk*)table, chunks, (double*)scratch);
     hipLaunchKernelGGL(grad_clip_kernel, dim3(1), dim3(256), 0, (hipStream_t)stream, (const double*)scratch, blocks, max_norm, clip);
     VINCE_CHECK_LAUNCH();
     return VINCE_OK;
@@ -266,7 +309,11 @@ extern "C" int vince_grad_scale(const void* table, int64_t chunks, const float* 
 
 extern "C" int vince_grad_clip(const void* table, int64_t chunks, float max_norm, float* clip, void* scratch, size_t scratch_bytes, void* stream) {
     GRAD_NORM_CHECK("vince_grad_clip");
-    if (chunks == 0) return vince_grad_norm(table, chunks, max_norm, clip, scratch, scratch_bytes, stream);
+    if (chunks <= SMALL_CHUNKS) {
+        hipLaunchKernelGGL(grad_small_kernel<true>, dim3(1), dim3(1024), 0, (hipStream_t)stream, (const GradChunk*)table, (int)chunks, max_norm, clip);
+        VINCE_CHECK_LAUNCH();
+        return VINCE_OK;
+    }
     const int blocks = blocks_of(chunks, GRAD_NORM_BLOCKS);
     hipLaunchKernelGGL(grad_squares_kernel, dim3(blocks), dim3(256), 0, (hipStream_t)stream, (const GradChunk*)table, chunks, (double*)scratch);
     hipLaunchKernelGGL(grad_scale_kernel<true>, dim3(blocks_of(chunks, GRAD_SCALE_BLOCKS)), dim3(256), 0, (hipStream_t)stream, (const GradChunk*)table, chunks, clip,

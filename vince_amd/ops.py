@@ -839,8 +839,10 @@ class GradTable:
         if not max_norm >= 0:
             raise ValueError("vince_amd: max_norm=%r" % (max_norm,))
         clip = torch.empty(2, device=self.device, dtype=torch.float32)
-        scratch = torch.empty(self._scratch_bytes, device=self.device, dtype=torch.uint8)    # (a call's own: two may be in flight)
-        self._run(fn, max_norm, clip.data_ptr(), scratch.data_ptr(), self._scratch_bytes)
+        scratch = None
+        if self._scratch_bytes:      # (a call's own: two may be in flight)
+            scratch = torch.empty(self._scratch_bytes, device=self.device, dtype=torch.uint8)
+        self._run(fn, max_norm, clip.data_ptr(), None if scratch is None else scratch.data_ptr(), self._scratch_bytes)
         return clip
 
 
