@@ -119,9 +119,9 @@ constexpr int block_threads(int tpr) { return tpr > 64 ? tpr : 256; }
 constexpr int wave_lanes(int tpr) { return tpr < 64 ? tpr : 64; }
 // the sum of a workgroup's per-wavefront values, one in each of 16 neighbouring lanes (0 behind the last wavefront)
 __device__ __forceinline__ float waves_sum(float v) { return lanes_sum<16>(v); }
-// Whether a thread keeps its columns' weight (and bias) in registers from row to row.  At 1024 threads, with 128 registers each, there is
-// room for 8 values only: else they are read again for every row, from the caches.
-constexpr bool holds_weights(int tpr, int values) { return tpr < 1024 || values <= 8; }
+// Whether a thread keeps its columns' weight (and bias) in registers from row to row.  Up to 1024 threads, with 128 registers each, there
+// is no room: they are read again for every row, from the caches (with room, at 2 fp32 chunks, holding them is 7 % slower all the same).
+constexpr bool holds_weights(int tpr) { return tpr < 1024; }
 
 // s / n from inv = 1 / n, with one step of correction: exact where the quotient is a float, so that a row of one value has that mean and
 // the bias as its output; a third of the instructions of a division, which every wavefront would make for every row
@@ -180,7 +180,7 @@ __global__ __launch_bounds__(block_threads(TPR)) void ln_fwd_kernel(const T* __r
                                                                     float* __restrict__ rstd, int64_t rows, int cols, float eps, int relu) {
     constexpr int V = Elem<T>::CH, R = TPR > 64 ? 1 : 256 / TPR, LANES = wave_lanes(TPR);
     constexpr bool WAVES = TPR > 64;                     // a row is several wavefronts'
-    constexpr bool HOLD = holds_weights(TPR, K * V);
+    constexpr bool HOLD = holds_weights(TPR);
     const int64_t stride = (int64_t)gridDim.x * R;
     int64_t row = (int64_t)blockIdx.x * R + (WAVES ? 0 : threadIdx.x / TPR);
     const Cols<T, TPR, K, MODE> at(cols, x + row * cols);
@@ -325,7 +325,7 @@ __global__ __launch_bounds__(block_threads(TPR)) void ln_bwd_kernel(const T* __r
                                                                     const T* __restrict__ dout, const T* __restrict__ act, T* __restrict__ dx,
                                                                     float* __restrict__ partial, int64_t rows, int cols) {
     constexpr int V = Elem<T>::CH, R = TPR > 64 ? 1 : 256 / TPR;
-    constexpr bool WAVES = TPR > 64, HOLD = holds_weights(TPR, K * V);
+    constexpr bool WAVES = TPR > 64, HOLD = holds_weights(TPR);
     const int64_t stride = (int64_t)gridDim.x * R;
     int64_t row = (int64_t)blockIdx.x * R + (WAVES ? 0 : threadIdx.x / TPR);
     const Cols<T, TPR, K, MODE> at(cols, x + row * cols);
@@ -679,7 +679,7 @@ __global__ __launch_bounds__(256) void ln_bwd_long_dw_kernel(const T* __restrict
 // Threads a row and chunks a thread, from the row's number of 16-byte chunks.  Up to 64 chunks: one a lane, the smallest power of two of
 // lanes (several rows share a wavefront).  Then a wavefront with up to KMAX a lane, then a workgroup of the wavefronts it takes, up to 16.
 // KMAX: what the registers hold with four wavefronts a SIMD -- 4 forward; backward, which keeps a weight and two sums a column, 16 values
-// (4 fp32 chunks, 2 bf16).  From 5 wavefronts on fp32 stops at 2: 16384 x 8192 takes 195 / 289 us forward / backward as 1024 threads of 2
+// (4 fp32 chunks, 2 bf16).  From 5 wavefronts on fp32 stops at 2: 16384 x 8192 takes 196 / 291 us forward / backward as 1024 threads of 2
 // chunks, 200 / 309 as 512 of 4 (bf16, 8192 x 16384 forward: 107 against 99, the other way).
 struct Split { int tpr, k, threads; int64_t chunks; bool shifted = false; };      // tpr, k: the kernel's; threads: a workgroup's
 Split ln_split(int dtype, int64_t chunks, int kmax) {

@@ -396,7 +396,7 @@ def _layer_norm_vector(what, name, v, cols):
 
 
 def layer_norm_fwd(x, weight=None, bias=None, eps=1e-5, relu=False):
-    """Layer norm over the last axis of x [..., D] (float32 or bfloat16): (x - mean) * rstd * weight + bias, rstd = 1 / sqrt(var + eps)
+    """Layer norm over the last axis of x [..., D] (float32 or bfloat16; no autograd): (x - mean) * rstd * weight + bias, rstd = 1 / sqrt(var + eps)
     with the biased variance; relu: max(., 0) in the same pass.  weight, bias: float32 [D] or None (no bias without a weight).
     Returns (out like x, mean float32 [...], rstd float32 [...]); layer_norm_bwd takes the last two."""
     index = _one_gpu(x, weight, bias)
