@@ -42,6 +42,27 @@ def test_layer_norm_refusals(L):
     assert bwd(rows=0, x=NULL, dout=NULL, dx=NULL, mean=NULL, rstd=NULL, acc=1) == 0
 
 
+def test_layer_norm_bwd_refuses_gradients_that_share_memory(L):
+    at = lambda bytes_off: ctypes.c_void_p(1 << 20 | bytes_off)  # noqa: E731
+    for rows, cols in ((4, 8), (4000, 64), (4, 40000)):          # one launch, two, long rows
+        need = L.vince_layer_norm_bwd_scratch_bytes(0, rows, cols)
+        for a, b in ((0, 0), (0, 4 * cols - 4), (4, 0)):
+            assert L.vince_layer_norm_bwd(0, PTR, PTR, PTR, PTR, PTR, NULL, PTR, at(a), at(b), 0, rows, cols, PTR, need, NULL) == -5
+            assert b"share memory" in L.vince_last_error()
+
+
+def test_longest_rows(L):
+    """The partial rows of a few very long rows are no more than the rows; a length past the C interface's 32 bits is refused, not cut."""
+    cols = 2 ** 31 - 1
+    for rows, parts in ((1, 1), (7, 7), (8, 8), (9, 8), (32, 8), (33, 16)):
+        assert L.vince_layer_norm_bwd_scratch_bytes(1, rows, cols) == parts * 2 * 4 * cols, rows
+    from vince_amd import ops
+    assert ops._layer_norm_shape("f", torch.empty(2, cols, device="meta"))[1] == cols
+    for n in (2 ** 31, 2 ** 32 + 8):
+        with pytest.raises(ValueError, match="2\\^31"):
+            ops._layer_norm_shape("f", torch.empty(2, n, device="meta"))
+
+
 def test_grad_entry_point_refusals(L):
     norm = lambda **k: L.vince_grad_norm(*[{**dict(table=PTR, chunks=300, limit=1.0, clip=PTR, scratch=PTR, nbytes=1 << 20, stream=NULL), **k}[n]  # noqa: E731
                                            for n in ("table", "chunks", "limit", "clip", "scratch", "nbytes", "stream")])

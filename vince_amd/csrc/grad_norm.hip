@@ -8,11 +8,13 @@ namespace {
 // Pieces of 2048 .. 16384 elements: small enough that a few hundred thousand elements reach every CU, large enough that the entries are
 // nothing beside what they list.
 constexpr int GRAD_CHUNK_MIN = 2048, GRAD_CHUNK_MAX = 16384;
+// Up to two pieces a wavefront of one workgroup (grad_small_kernel).  us of a clipping call in that one launch / in two, 16, 32 and 64
+// pieces: on an idle device 8.0 / 8.9, 10.9 / 8.9, 15.8 / 8.9; calls back to back, where a launch counts, 3.7 / 7.1, 4.4 / 7.2, 6.7 / 7.2.
+constexpr int SMALL_CHUNKS = 32;
 // Workgroups: 8 MB of loads in flight where only gradients are read, 4 MB where they are written back too, 6 MB in the SGD step's three
 // streams.  us at 256 / 512 / 1024 / 2048 of them, 160 M fp32: norm 126 / 103 / 107 / 112 (6.2 TB/s at 512), scaling 219 / 244 / 246 / 247;
 // norm and SGD step of 28 M at 256 / 512: 120 / 112.  (A piece's entry is read when the piece begins: read ahead, scaling takes 247 us at
 // 256, the norm 107 at 512.)
-constexpr int SMALL_CHUNKS = 64;
 constexpr int GRAD_NORM_BLOCKS = 512, GRAD_SCALE_BLOCKS = 256, SGD_BLOCKS = 512;
 constexpr uint32_t GRAD_BF16 = 1u << 31;
 

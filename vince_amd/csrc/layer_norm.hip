@@ -721,11 +721,12 @@ int64_t ln_fwd_blocks(int64_t rows, const Split& s) {
     const int64_t r = s.tpr && s.tpr <= 64 ? 256 / s.tpr : 1, want = (rows + r - 1) / r, most = ln_blocks(s, 1 << 18);
     return want < most ? want : most;
 }
-// (at least four rows for each row group, so that the partial rows stay a small part of what is read)
+// (at least four rows for each row group, so that the partial rows stay a small part of what is read; of the longest rows, which can be
+// gigabytes, no more partial rows than rows)
 int ln_bwd_blocks(int64_t rows, const Split& s) {
     const int64_t per = s.tpr && s.tpr <= 64 ? 4 * (256 / s.tpr) : 4, most = s.tpr ? ln_blocks(s, 1 << 17) : 256;
     const int64_t n = ((rows + per - 1) / per + 7) / 8 * 8;
-    return (int)(n > most ? most : n);
+    return (int)(!s.tpr && n > rows ? rows : n > most ? most : n);
 }
 // Few rows (ln_bwd_few_kernel): one launch for two and no scratch, against reading x and dout twice and column sums that one workgroup makes
 // over all rows.  us of a call, two launches / one: 256 x 2048 fp32 8.4 / 5.3, 512 x 8192 bf16 14.7 / 9.9, 1024 x 512 fp32 8.1 / 5.7, 1024 x
@@ -825,7 +826,7 @@ template <typename T> void run_bwd(const Split& s, const BwdArgs& a, hipStream_t
     hipLaunchKernelGGL(ln_bwd_long_dx_kernel<T>, dim3((unsigned)(a.rows < 1024 ? a.rows : 1024)), dim3(1024), 0, st, (const T*)a.x, a.w, a.mean,
                        a.rstd, (const T*)a.dout, (const T*)a.act, (T*)a.dx, a.rows, a.cols);
     if (a.dw)
-        hipLaunchKernelGGL(ln_bwd_long_dw_kernel<T>, dim3((unsigned)((a.cols + 256 * Elem<T>::CH - 1) / (256 * Elem<T>::CH)), (unsigned)a.blocks),
+        hipLaunchKernelGGL(ln_bwd_long_dw_kernel<T>, dim3((unsigned)((a.cols + (int64_t)(256 * Elem<T>::CH - 1)) / (256 * Elem<T>::CH)), (unsigned)a.blocks),
                            dim3(256), 0, st, (const T*)a.x, a.mean, a.rstd, (const T*)a.dout, (const T*)a.act, a.partial, a.rows, a.cols);
 }
 
@@ -865,6 +866,8 @@ extern "C" int vince_layer_norm_bwd(int dtype, const void* x, const float* weigh
         VINCE_CHECK_ARG(x && mean && rstd && dout && dx, VINCE_E_ARG, "vince_layer_norm_bwd: null pointer");
         const size_t need = dweight ? vince_layer_norm_bwd_scratch_bytes(dtype, rows, cols) : 0;
         VINCE_CHECK_ARG(need == 0 || (scratch && scratch_bytes >= need), VINCE_E_ARG, "vince_layer_norm_bwd: scratch of %zu bytes", scratch_bytes);
+        const uintptr_t dw = (uintptr_t)dweight, db = (uintptr_t)dbias, bytes = (uintptr_t)cols * sizeof(float);
+        VINCE_CHECK_ARG(!dweight || dw + bytes <= db || db + bytes <= dw, VINCE_E_ARG, "vince_layer_norm_bwd: dweight and dbias share memory");
         const BwdArgs a = {x, dout, act, weight, mean, rstd, dx, dweight, dbias, few || !dweight ? nullptr : (float*)scratch, accumulate, rows, cols, blocks, s.threads, s.shifted};
         if (dtype == VINCE_F32) run_bwd<float>(s, a, st);
         else run_bwd<bf16_t>(s, a, st);

@@ -386,6 +386,8 @@ def l2norm_bwd(x, norms, dout, eps=1e-12):
 def _layer_norm_shape(what, x):
     if x.dim() == 0 or x.shape[-1] == 0:
         raise ValueError("%s: x has no last axis to normalise, got shape %s" % (what, tuple(x.shape)))
+    if x.shape[-1] > 2 ** 31 - 1:
+        raise ValueError("%s: rows of %d values, at most 2^31 - 1" % (what, x.shape[-1]))
     return dtype_code(x), x.shape[-1]
 
 
