@@ -135,6 +135,16 @@ def test_layer_norm_rows(rows, cols, dtype):
     check_bwd(x, w, mean, rstd, randn(rows, cols, seed=3, dtype=dtype))
 
 
+@pytest.mark.parametrize("rows", [7, 1031])
+@pytest.mark.parametrize("cols", [4099, 4352, 5000, 5120, 5121, 6143, 6144, 6145, 6400])
+def test_layer_norm_rows_of_five_to_seven_wavefronts(cols, rows):
+    """fp32 rows around the length from which a thread has two chunks instead of four: whole and cut ones, few and many."""
+    x = randn(rows, cols, seed=cols) + 0.25
+    w, b = 1 + 0.2 * randn(cols, seed=1), 0.3 * randn(cols, seed=2)
+    act, mean, rstd = check_fwd(x, w, b, relu=True)
+    check_bwd(x, w, mean, rstd, randn(rows, cols, seed=3), act=act)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_layer_norm_without_parameters_and_with_leading_axes(dtype):
     x = randn(3, 5, 7, 96, seed=4, dtype=dtype)

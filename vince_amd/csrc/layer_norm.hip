@@ -679,8 +679,9 @@ __global__ __launch_bounds__(256) void ln_bwd_long_dw_kernel(const T* __restrict
 // Threads a row and chunks a thread, from the row's number of 16-byte chunks.  Up to 64 chunks: one a lane, the smallest power of two of
 // lanes (several rows share a wavefront).  Then a wavefront with up to KMAX a lane, then a workgroup of the wavefronts it takes, up to 16.
 // KMAX: what the registers hold with four wavefronts a SIMD -- 4 forward; backward, which keeps a weight and two sums a column, 16 values
-// (4 fp32 chunks, 2 bf16).  From 5 wavefronts on fp32 stops at 2: 16384 x 8192 takes 196 / 291 us forward / backward as 1024 threads of 2
-// chunks, 200 / 309 as 512 of 4 (bf16, 8192 x 16384 forward: 107 against 99, the other way).
+// (4 fp32 chunks, 2 bf16).  From 7 wavefronts on fp32 stops at 2: 16384 x 8192 takes 194 / 291 us forward / backward as 1024 threads of 2
+// chunks, 201 / 310 as 512 of 4, 20000 x 7000 takes 211 / 332 and 216 / 329; with 5 and 6 it is the other way, 20000 x 5000 157 / 238 and
+// 141 / 227, 20000 x 6000 186 / 270 and 181 / 273 (bf16, 8192 x 16384 forward: 107 against 99).
 struct Split { int tpr, k, threads; int64_t chunks; bool shifted = false; };      // tpr, k: the kernel's; threads: a workgroup's
 Split ln_split(int dtype, int64_t chunks, int kmax) {
     if (chunks <= 64) {
@@ -689,7 +690,7 @@ Split ln_split(int dtype, int64_t chunks, int kmax) {
         return {tpr, 1, 256, chunks};
     }
     for (int tpr = 64; tpr <= 1024; tpr = tpr == 64 ? 256 : tpr * 2)
-        for (int k = 1; k <= (dtype == VINCE_F32 && tpr == 512 ? 2 : kmax); k *= 2)
+        for (int k = 1; k <= (dtype == VINCE_F32 && tpr == 512 && chunks > 1536 ? 2 : kmax); k *= 2)
             if ((int64_t)tpr * k >= chunks) return {tpr, k, tpr == 64 ? 256 : (int)((chunks + 64 * k - 1) / (64 * k)) * 64, chunks};
     return {0, 0, 0, chunks};
 }
@@ -762,9 +763,8 @@ void run_fwd(int dtype, const void* x, const float* w, const float* b, void* out
 #define LN_CASE(TPR, K) \
     if (s.tpr == TPR && s.k == K) return launch_fwd<T, TPR, K>(s.shifted, grid, block, x, w, b, out, mean, rstd, rows, cols, eps, relu, st)
     LN_CASE(2, 1); LN_CASE(4, 1); LN_CASE(8, 1); LN_CASE(16, 1); LN_CASE(32, 1); LN_CASE(64, 1); LN_CASE(64, 2); LN_CASE(64, 4);
-    LN_CASE(256, 2); LN_CASE(256, 4); LN_CASE(1024, 4);
+    LN_CASE(256, 2); LN_CASE(256, 4); LN_CASE(512, 4); LN_CASE(1024, 4);
     if constexpr (sizeof(T) == 4) { LN_CASE(1024, 2); }
-    else { LN_CASE(512, 4); }
 #undef LN_CASE
     hipLaunchKernelGGL(ln_fwd_long_kernel<T>, grid, dim3(1024), 0, st, (const T*)x, w, b, (T*)out, mean, rstd,
                        rows, cols, eps, relu);
@@ -818,7 +818,7 @@ template <typename T> void run_bwd(const Split& s, const BwdArgs& a, hipStream_t
     if (s.tpr == TPR && s.k == K) return launch_bwd<T, TPR, K>(a, st)
     LN_CASE(2, 1); LN_CASE(4, 1); LN_CASE(8, 1); LN_CASE(16, 1); LN_CASE(32, 1); LN_CASE(64, 1); LN_CASE(64, 2); LN_CASE(256, 2);
     if constexpr (sizeof(T) == 4) {
-        LN_CASE(64, 4); LN_CASE(256, 4); LN_CASE(1024, 2); LN_CASE(1024, 4);
+        LN_CASE(64, 4); LN_CASE(256, 4); LN_CASE(512, 4); LN_CASE(1024, 2); LN_CASE(1024, 4);
     } else {
         LN_CASE(256, 1); LN_CASE(512, 2); LN_CASE(1024, 2);
     }
