@@ -730,10 +730,11 @@ int ln_bwd_blocks(int64_t rows, const Split& s) {
     return (int)(!s.tpr && n > rows ? rows : n > most ? most : n);
 }
 // Few rows (ln_bwd_few_kernel): one launch for two and no scratch, against reading x and dout twice and column sums that one workgroup makes
-// over all rows.  us of a call, two launches / one: 256 x 2048 fp32 8.4 / 5.3, 512 x 8192 bf16 14.7 / 9.9, 1024 x 512 fp32 8.1 / 5.7, 1024 x
-// 2048 bf16 9.0 / 10.0 (and 2 us for the scratch's allocation).
+// over all rows.  us of a call, two launches / one: 256 x 2048 fp32 8.4 / 5.3, 512 x 8192 bf16 12.4 / 10.8, 512 x 16384 fp32 32.0 / 28.1, 512 x
+// 8192 fp32 15.6 / 16.5; 1024 x 512 fp32 8.1 / 5.7, 1024 x 2048 bf16 9.0 / 10.0, 1000 x 4096 fp32 13.8 / 15.1 (and 2 us for the scratch's
+// allocation).
 bool ln_bwd_few(int dtype, int64_t rows, int cols) {
-    return ln_few_split(dtype, cols).tpr && rows <= 1024 && rows * ln_chunks(dtype, cols) <= (rows <= 512 ? 1 << 19 : 1 << 18);
+    return ln_few_split(dtype, cols).tpr && (rows <= 512 || (rows <= 1024 && rows * ln_chunks(dtype, cols) <= 1 << 18));
 }
 
 template <typename T, int TPR, int K>
