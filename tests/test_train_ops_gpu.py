@@ -321,6 +321,39 @@ def test_layer_norm_rows_past_32_bit_offsets():
     inside(db, want, bound, "dbias")
 
 
+@pytest.mark.parametrize("rows", [0, 1, 3])
+@pytest.mark.parametrize("cols", [(1 << 25) + 1, (1 << 26) - 1, (1 << 26) + 1])
+def test_layer_norm_bwd_of_very_long_rows(cols, rows):
+    """dweight and dbias on both sides of the length at which a workgroup for every 32 of their columns would be 2^32 threads, which no
+    launch has; no rows: their sum is 0.  mean and rstd are given, so that one row's dweight is a difference and two products."""
+    dtype = torch.bfloat16
+    x, dout = randn(rows, cols, seed=1, dtype=dtype), randn(rows, cols, seed=2, dtype=dtype)
+    mean, rstd = torch.tensor([0.25, -0.5, 0.0], device=DEV)[:rows], torch.tensor([1.5, 0.75, 1.0], device=DEV)[:rows]
+    dw, db = _ops().layer_norm_bwd(x, torch.ones(cols, device=DEV), mean, rstd, dout)[1:]
+    xh = (x.float() - mean[:, None]) * rstd[:, None]
+    # a difference, a product, a multiply-add a row, the partial rows' additions
+    for name, got, terms in (("dweight", dw, dout.double() * xh.double()), ("dbias", db, dout.double())):
+        inside(got, terms.sum(0), (rows + 4) * U * terms.abs().sum(0), name)
+
+
+def test_layer_norm_bwd_of_the_longest_row():
+    """2^31 - 1 columns: every column of dweight and dbias, added to what was there (128 million at a time)."""
+    cols, step = (1 << 31) - 1, 1 << 27
+    x = torch.empty(1, cols, device=DEV, dtype=torch.bfloat16)
+    dout = torch.empty_like(x)
+    for i in range(0, cols, step):
+        n = min(step, cols - i)
+        x[0, i:i + n] = randn(n, seed=i % 1000003, dtype=torch.bfloat16)
+        dout[0, i:i + n] = randn(n, seed=i % 1000003 + 1, dtype=torch.bfloat16)
+    mean, rstd = torch.tensor([0.25], device=DEV), torch.tensor([1.5], device=DEV)
+    dw, db = torch.full((cols,), 2.0, device=DEV), torch.full((cols,), -3.0, device=DEV)
+    _ops().layer_norm_bwd(x, torch.ones(cols, device=DEV), mean, rstd, dout, dweight=dw, dbias=db)
+    for i in range(0, cols, step):
+        d, xh = dout[0, i:i + step].double(), (x[0, i:i + step].double() - 0.25) * 1.5
+        inside(dw[i:i + step], 2 + d * xh, 4 * U * (d * xh).abs() + U * (2 + d * xh).abs() * 1.01, "dweight")
+        inside(db[i:i + step], d - 3, U * (d - 3).abs(), "dbias")
+
+
 def test_layer_norm_gradients_against_differences():
     """dx, dweight and dbias of sum(c * y) against central differences of the forward formula in 64 bits; and of the kernel's own
     forward along random directions."""

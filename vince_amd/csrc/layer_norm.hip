@@ -507,31 +507,37 @@ __global__ __launch_bounds__(block_threads(TPR)) void ln_bwd_few_kernel(const T*
     }
 }
 
-// dweight / dbias = (or +=) the sum of `parts` partial rows [2][cols]: 32 columns x 32 rows at a time, the rows' sums in a fixed order
+// dweight / dbias = (or +=) the sum of `parts` partial rows [2][cols]: 32 columns x 32 rows at a time, the rows' sums in a fixed order.
+// Up to JOIN_BLOCKS workgroups of 32 columns, each of which has one turn below 2^25 columns: HIP launches less than 2^32 threads along an
+// axis, which a workgroup for every 32 of the longest rows' columns would pass from 2^26 columns on.
+constexpr int JOIN_BLOCKS = 1 << 21;
 __global__ __launch_bounds__(1024) void ln_bwd_join_kernel(const float* __restrict__ partial, int parts, int64_t cols2, int cols,
                                                            float* __restrict__ dw, float* __restrict__ db, int accumulate) {
     __shared__ float red[32][33];
     const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-    const int64_t c = (int64_t)blockIdx.x * 32 + tx;
-    float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
-    if (c < cols2) {
-        const float* p = partial + c;
-        int i = ty;
-        for (; i + 96 < parts; i += 128) {
-            const float a0 = p[(int64_t)i * cols2], a1 = p[(int64_t)(i + 32) * cols2], a2 = p[(int64_t)(i + 64) * cols2],
-                        a3 = p[(int64_t)(i + 96) * cols2];
-            s0 += a0; s1 += a1; s2 += a2; s3 += a3;
+    for (int64_t c0 = (int64_t)blockIdx.x * 32; c0 < cols2; c0 += (int64_t)gridDim.x * 32) {      // (the same turns for a whole workgroup)
+        const int64_t c = c0 + tx;
+        float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+        if (c < cols2) {
+            const float* p = partial + c;
+            int i = ty;
+            for (; i + 96 < parts; i += 128) {
+                const float a0 = p[(int64_t)i * cols2], a1 = p[(int64_t)(i + 32) * cols2], a2 = p[(int64_t)(i + 64) * cols2],
+                            a3 = p[(int64_t)(i + 96) * cols2];
+                s0 += a0; s1 += a1; s2 += a2; s3 += a3;
+            }
+            for (; i < parts; i += 32) s0 += p[(int64_t)i * cols2];
         }
-        for (; i < parts; i += 32) s0 += p[(int64_t)i * cols2];
-    }
-    red[ty][tx] = (s0 + s1) + (s2 + s3);
-    __syncthreads();
-    if (ty == 0 && c < cols2) {
-        float s = 0.f;
+        red[ty][tx] = (s0 + s1) + (s2 + s3);
+        __syncthreads();
+        if (ty == 0 && c < cols2) {
+            float s = 0.f;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) s += red[i][tx];
-        float* out = c < cols ? dw + c : db + (c - cols);
-        *out = accumulate ? *out + s : s;
+            for (int i = 0; i < 32; ++i) s += red[i][tx];
+            float* out = c < cols ? dw + c : db + (c - cols);
+            *out = accumulate ? *out + s : s;
+        }
+        __syncthreads();                   // (before the next turn writes red)
     }
 }
 
@@ -875,7 +881,8 @@ extern "C" int vince_layer_norm_bwd(int dtype, const void* x, const float* weigh
         VINCE_CHECK_LAUNCH();
     }
     if (dweight && !few && (rows > 0 || !accumulate)) {
-        hipLaunchKernelGGL(ln_bwd_join_kernel, dim3((unsigned)((2 * (int64_t)cols + 31) / 32)), dim3(1024), 0, st, (const float*)scratch,
+        const int64_t groups = (2 * (int64_t)cols + 31) / 32;
+        hipLaunchKernelGGL(ln_bwd_join_kernel, dim3((unsigned)(groups < JOIN_BLOCKS ? groups : JOIN_BLOCKS)), dim3(1024), 0, st, (const float*)scratch,
                            rows > 0 ? blocks : 0, 2 * (int64_t)cols, cols, dweight, dbias, accumulate);
         VINCE_CHECK_LAUNCH();
     }
