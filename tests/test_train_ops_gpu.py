@@ -354,6 +354,58 @@ def test_layer_norm_bwd_of_the_longest_row():
         inside(db[i:i + step], d - 3, U * (d - 3).abs(), "dbias")
 
 
+@pytest.mark.parametrize("value", [0.3, 1 / 3])
+@pytest.mark.parametrize("cols", [40000, (1 << 25) + 3, 1 << 27])
+def test_layer_norm_long_rows_of_one_value(cols, value):
+    """Rows past a workgroup's registers, of one value that fp32 sums of a few hundred thousand of it do not hold: the mean is that value
+    (chunks of four are exact, their fp64 sum has at most 24 + 25 bits, a cut chunk's one rounding is below 2^-24 / cols of the sum), the
+    output the bias."""
+    x = torch.full((1, cols), value, device=DEV)
+    b = randn(cols, seed=3)
+    out, mean, rstd = _ops().layer_norm_fwd(x, torch.ones(cols, device=DEV), b)
+    assert torch.equal(mean, x[:, 0]) and torch.equal(out[0], b)
+    want = torch.full((1,), float(np.float32(1e-5)), device=DEV, dtype=torch.float64).rsqrt()
+    inside(rstd, want, 1.01 * U * want, "rstd")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("cols", [40001, (1 << 25) + 5])
+def test_layer_norm_long_rows_are_as_good_as_short_ones(cols, dtype):
+    """Bounds that do not grow with the row's length: sums of 8 values in a tree of three fp32 additions (3 u of the magnitudes), fp64
+    sums of those.  Backward with a level dout, whose average c1 takes out of dx."""
+    x = (randn(2, cols, seed=1) + torch.tensor([[0.5], [-2.0]], device=DEV)).to(dtype)
+    w, b = 1 + 0.2 * randn(cols, seed=2), 0.3 * randn(cols, seed=3)
+    out, mean, rstd = _ops().layer_norm_fwd(x, w, b)
+    X, W = x.double(), w.double()
+    m = X.mean(1, keepdim=True)
+    xc = X - m
+    var = (xc * xc).mean(1, keepdim=True)
+    r = (var + float(np.float32(1e-5))).rsqrt()
+    dm = 3.01 * U * X.abs().mean(1, keepdim=True) + 1.01 * U * m.abs()
+    inside(mean[:, None], m, dm, "mean")
+    # squares: twice the centred value's rounding and the mean's, the product's, the tree's; the mean's error has no first order in the sum
+    dvar = 4.1 * U * var + dm * dm + 2.02 * U * (xc.abs() * (xc.abs() + dm)).mean(1, keepdim=True)
+    dr = r * (0.5 * dvar / (var + 1e-5) * 1.01 + 1.01 * U)
+    inside(rstd[:, None], r, dr, "rstd")
+    xh = xc * r
+    y = xh * W + b.double()
+    dy = ((r * (dm + U * xc.abs()) + xc.abs() * dr + U * xh.abs()) * W.abs() + U * y.abs()) * 1.01
+    inside(out, y, dy + (y.abs() + dy) * STORE[dtype] + TINY, "out")
+    dout = torch.full_like(x, 0.3)
+    dx, dw, db = _ops().layer_norm_bwd(x, w, mean, rstd, dout)
+    G, m, r = dout.double(), mean.double()[:, None], rstd.double()[:, None]
+    xh = (X - m) * r
+    g = G * W
+    c1, c2 = g.mean(1, keepdim=True), (g * xh).mean(1, keepdim=True)
+    d1 = 5 * U * g.abs().mean(1, keepdim=True)                       # g's rounding, the tree, c1's own
+    d2 = 8 * U * (g * xh).abs().mean(1, keepdim=True)                # xhat's two and g's, the product, the tree, c2's own
+    want = r * (g - c1 - xh * c2)
+    bound = r * (3 * U * g.abs() + d1 + 4 * U * c1.abs() + xh.abs() * d2 + 6 * U * (xh * c2).abs()) * 1.01 + 2 * U * want.abs()
+    inside(dx, want, bound + (want.abs() + bound) * STORE[dtype] + TINY, "dx")
+    inside(dw, (G * xh).sum(0), 7 * U * (G * xh).abs().sum(0), "dweight")         # xhat's two, two multiply-adds, the join's
+    inside(db, G.sum(0), 4 * U * G.abs().sum(0), "dbias")
+
+
 def test_layer_norm_gradients_against_differences():
     """dx, dweight and dbias of sum(c * y) against central differences of the forward formula in 64 bits; and of the kernel's own
     forward along random directions."""
