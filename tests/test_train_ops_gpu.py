@@ -135,6 +135,36 @@ def test_layer_norm_rows(rows, cols, dtype):
     check_bwd(x, w, mean, rstd, randn(rows, cols, seed=3, dtype=dtype))
 
 
+# a whole and a cut length (bfloat16: an even and an odd one) for every number of threads a row and of chunks a thread that the forward and
+# the backward of many rows take
+MANY = {torch.float32: [5, 8, 13, 16, 21, 32, 50, 64, 99, 128, 201, 256, 400, 512, 770, 1024, 1300, 1536, 2047, 2048, 3001, 4096, 4101, 5120,
+                        6656, 7003, 8192, 8197, 9216, 12001, 16384],
+        torch.bfloat16: [9, 16, 17, 22, 27, 32, 40, 59, 64, 100, 123, 128, 200, 251, 256, 400, 507, 512, 900, 1019, 1024, 1500, 1536, 2043, 2048,
+                         2100, 4091, 4096, 5000, 5120, 8187, 8192, 9216, 10000, 16377, 16384]}
+
+
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("dtype,cols", [(t, c) for t in DTYPES for c in MANY[t]])
+def test_layer_norm_many_rows(cols, dtype, masked):
+    """More rows than one turn of the workgroups takes, and more than the backward of few rows is for: its partial rows go through
+    scratch, which a call of the other kind would not ask for."""
+    from vince_amd import _lib
+    ops = _ops()
+    w, b = 1 + 0.2 * randn(cols, seed=1), 0.3 * randn(cols, seed=2)
+    for rows in (1031, 6007) if cols <= 1024 else (1031,):
+        x = (randn(rows, cols, seed=rows + cols) * (0.5 + torch.arange(rows, device=DEV)[:, None] % 7) + 0.5).to(dtype)
+        assert _lib.lib().vince_layer_norm_bwd_scratch_bytes(ops.dtype_code(x), rows, cols) > 0
+        act, mean, rstd = check_fwd(x, w, b, relu=masked)
+        check_bwd(x, w, mean, rstd, randn(rows, cols, seed=3, dtype=dtype), act=act if masked else None)
+
+
+@pytest.mark.parametrize("cols", [16379, 16386, 18432, 20000, 20011, 32761, 32766, 32767, 32768])
+def test_layer_norm_many_rows_of_the_forward_alone(cols):
+    """bfloat16 rows that the forward's registers still hold and the backward's do not."""
+    x = (randn(517, cols, seed=cols) * (0.5 + torch.arange(517, device=DEV)[:, None] % 7) + 0.5).bfloat16()
+    check_fwd(x, 1 + 0.2 * randn(cols, seed=1), 0.3 * randn(cols, seed=2), relu=cols % 2 == 0)
+
+
 @pytest.mark.parametrize("rows", [7, 1031])
 @pytest.mark.parametrize("cols", [4099, 4352, 5000, 5120, 5121, 6143, 6144, 6145, 6400])
 def test_layer_norm_rows_of_five_to_seven_wavefronts(cols, rows):
