@@ -544,7 +544,8 @@ int vince_colsum(const float* x, float* out, int32_t rows, int32_t cols, void* s
  *     dweight = sum over the rows of d xhat, dbias = sum of d (accumulate != 0: added to what is there), fixed order of summation.
  *     dweight and dbias may both be NULL.  scratch: vince_layer_norm_bwd_scratch_bytes(), not read before it is written.
  * No alignment beyond the element's is needed, rows may be 0 (cols >= 1), a value that is not finite spoils its own row (and its
- * columns' sums) only.  No output may share memory with an input or another output.  (ABI 13) */
+ * columns' sums) only.  Sums are fp32 (over rows past the registers fp64 between 16-byte chunks): values whose sum, or whose squares
+ * about the mean, pass fp32's range in one row (|x| of 1e18 in a row of a few hundred) overflow as infinite ones would.  No output may share memory with an input or another output.  (ABI 13) */
 int vince_layer_norm_fwd(int dtype, const void* x, const float* weight, const float* bias, void* out, float* mean, float* rstd,
                          int64_t rows, int32_t cols, float eps, int32_t relu, void* stream);
 size_t vince_layer_norm_bwd_scratch_bytes(int dtype, int64_t rows, int32_t cols);

@@ -8,13 +8,12 @@ namespace {
 // Pieces of 2048 .. 16384 elements: small enough that a few hundred thousand elements reach every CU, large enough that the entries are
 // nothing beside what they list.
 constexpr int GRAD_CHUNK_MIN = 2048, GRAD_CHUNK_MAX = 16384;
-// Up to two pieces a wavefront of one workgroup (grad_small_kernel).  us of a clipping call in that one launch / in two, 16, 32 and 64
-// pieces: on an idle device 8.0 / 8.9, 10.9 / 8.9, 15.8 / 8.9; calls back to back, where a launch counts, 3.7 / 7.1, 4.4 / 7.2, 6.7 / 7.2.
+// Up to two pieces a wavefront of one workgroup (grad_small_kernel).  us on the device of clipping in that one launch / in two, 16, 32 and
+// 64 pieces of 2048 fp32 values: 3.8 / 5.0, 4.9 / 5.1, 7.2 / 5.1.
 constexpr int SMALL_CHUNKS = 32;
 // Workgroups: 8 MB of loads in flight where only gradients are read, 4 MB where they are written back too, 6 MB in the SGD step's three
-// streams.  us at 256 / 512 / 1024 / 2048 of them, 160 M fp32: norm 126 / 103 / 107 / 112 (6.2 TB/s at 512), scaling 219 / 244 / 246 / 247;
-// norm and SGD step of 28 M at 256 / 512: 120 / 112.  (A piece's entry is read when the piece begins: read ahead, scaling takes 247 us at
-// 256, the norm 107 at 512.)
+// streams.  us at 256 / 512 / 1024 / 2048 of them, 160 M fp32: norm 128 / 109 / 110 / 113 (5.9 TB/s at 512), scaling 226 / 253 / 249 / 248;
+// norm and SGD step of 28 M 123 / 113 / 118 / 118.
 constexpr int GRAD_NORM_BLOCKS = 512, GRAD_SCALE_BLOCKS = 256, SGD_BLOCKS = 512;
 constexpr uint32_t GRAD_BF16 = 1u << 31;
 
@@ -203,8 +202,8 @@ __global__ __launch_bounds__(1024) void grad_small_kernel(const GradChunk* __res
 
 // sgd_kernel (misc.hip) with the scale of the gradient taken from device memory: the same operations in the same order.  The momentum
 // passes the Infinity Cache by (non-temporal both ways; nothing reads it before the next step), which leaves the gradients there that the
-// norm has just read, and the parameters for the average and the weight copies that follow: norm and step of 28 M parameters 122 -> 112 us,
-// with the key encoder's average behind them 175 -> 166.
+// norm has just read, and the parameters for the average and the weight copies that follow: norm and step of 28 M parameters 124 -> 113 us,
+// with the key encoder's average behind them 176 -> 167.
 typedef __attribute__((ext_vector_type(4))) float f32x4_nt_t;
 __global__ __launch_bounds__(256) void sgd_clip_kernel(float* __restrict__ p, const float* __restrict__ g, float* __restrict__ buf, int64_t n,
                                                        float lr, float mom, float wd, float grad_scale, const float* __restrict__ clip) {

@@ -120,7 +120,8 @@ constexpr int wave_lanes(int tpr) { return tpr < 64 ? tpr : 64; }
 // the sum of a workgroup's per-wavefront values, one in each of 16 neighbouring lanes (0 behind the last wavefront)
 __device__ __forceinline__ float waves_sum(float v) { return lanes_sum<16>(v); }
 // Whether a thread keeps its columns' weight (and bias) in registers from row to row.  Up to 1024 threads, with 128 registers each, there
-// is no room: they are read again for every row, from the caches (with room, at 2 fp32 chunks, holding them is 7 % slower all the same).
+// is no room: they are read again for every row, from the caches (held, 16384 x 8192 fp32 takes 205 / 313 us forward / backward instead of
+// 200 / 292, 16384 x 16384 392 / 676 instead of 400 / 586).
 constexpr bool holds_weights(int tpr) { return tpr < 1024; }
 
 // s / n from inv = 1 / n, with one step of correction: exact where the quotient is a float, so that a row of one value has that mean and
@@ -132,9 +133,12 @@ __device__ __forceinline__ float divide(float s, float n, float inv) {
 
 // How the rows lie.  FULL: cols == TPR * K * V, every chunk whole.  PLAIN: the chunks start with the row, the first K / 2 are whole
 // (ln_split takes K > 1 for rows of more than TPR * K / 2 chunks).  SHIFTED: bfloat16 rows of an odd length start at every other address;
-// a 16-byte access that is not even aligned to 4 bytes occupies the vector cache three times as long (PMC: 49 M accesses for 15 M in the
-// backward of 65536 x 2047 against 2048), so the chunks start at the 16-byte boundaries of memory, the first before the row.  A thread's
-// rows are a multiple of 8 apart (the grid's size is, where it has more than one): the boundaries are the same in each.
+// a 16-byte access that is not even aligned to 4 bytes occupies the vector cache three times as long (PMC: 47 M accesses for 13 M in the
+// backward of 65536 x 2047 against 2048; 31 M shifted), so the chunks start at the 16-byte boundaries of memory, the first before the row.
+// A thread's rows are a multiple of 8 apart (the grid's size is, where it has more than one): the boundaries are the same in each.  us
+// PLAIN / SHIFTED: 65536 x 2049 forward 129 / 116, backward 219 / 191; 32768 x 4095 127 / 120 and 212 / 168; 65536 x 2047 98 / 118 and 210 /
+// 192, 16384 x 8191 136 / 104 and 192 / 203 -- below a power of two the row has a chunk more than one wavefront (2047 forward) or the
+// workgroups with room for their weights (8191 backward) hold.
 enum Mode { FULL, PLAIN, SHIFTED };
 
 // This thread's K chunks of a row.
@@ -717,9 +721,9 @@ __global__ __launch_bounds__(256) void ln_bwd_long_dw_kernel(const T* __restrict
 // Threads a row and chunks a thread, from the row's number of 16-byte chunks.  Up to 64 chunks: one a lane, the smallest power of two of
 // lanes (several rows share a wavefront).  Then a wavefront with up to KMAX a lane, then a workgroup of the wavefronts it takes, up to 16.
 // KMAX: what the registers hold with four wavefronts a SIMD -- 4 forward; backward, which keeps a weight and two sums a column, 16 values
-// (4 fp32 chunks, 2 bf16).  From 7 wavefronts on fp32 stops at 2: 16384 x 8192 takes 194 / 291 us forward / backward as 1024 threads of 2
-// chunks, 201 / 310 as 512 of 4, 20000 x 7000 takes 211 / 332 and 216 / 329; with 5 and 6 it is the other way, 20000 x 5000 157 / 238 and
-// 141 / 227, 20000 x 6000 186 / 270 and 181 / 273 (bf16, 8192 x 16384 forward: 107 against 99).
+// (4 fp32 chunks, 2 bf16).  From 7 wavefronts on fp32 stops at 2: 16384 x 8192 takes 200 / 293 us forward / backward as 1024 threads of 2
+// chunks, 208 / 311 as 512 of 4, 20000 x 7000 takes 212 / 335 and 219 / 328; with 5 and 6 it is the other way, 20000 x 5000 157 / 242 and
+// 143 / 224, 20000 x 6000 189 / 275 and 182 / 274.
 struct Split { int tpr, k, threads; int64_t chunks; bool shifted = false; };      // tpr, k: the kernel's; threads: a workgroup's
 Split ln_split(int dtype, int64_t chunks, int kmax) {
     if (chunks <= 64) {
@@ -749,9 +753,9 @@ Split ln_few_split(int dtype, int cols) { return ln_plain_split(dtype, cols, ln_
 
 // Workgroups: as many as have 4 MB of rows in their registers -- 2^18 chunks, of one tensor forward, of two backward -- and one a CU at
 // least; each goes through its share of the rows.  More rows at a time are slower, fewer too (forward, 65536 x 2048 bf16, us at 256 / 512
-// / 1024 / 2048 workgroups of 4 chunks a thread: 91 / 98 / 99 / 97; 10^6 x 128, of 1: 188 / 113 / 88 / 104; backward, 32768 x 4096, of 2:
-// 144 / 150 / 172 at 256 / 512 / 1024, where every workgroup also leaves a partial row of 8 bytes a column to be read again).  The same
-// number for every CU: 60000 x 1000 bf16 takes 44 us with 512, 50 with 520.  (Any multiple of 8 would do for Mode.)
+// / 1024 / 2048 workgroups of 4 chunks a thread: 94 / 100 / 101 / 99; 10^6 x 128, of 1: 194 / 116 / 91 / 103; backward, 32768 x 4096, of 2:
+// 142 / 152 / 176 at 256 / 512 / 1024, where every workgroup also leaves a partial row of 8 bytes a column to be read again).  The same
+// number for every CU: 60000 x 1000 bf16 takes 39 us with 512, 44 with 520.  (Any multiple of 8 would do for Mode.)
 int64_t ln_blocks(const Split& s, int64_t in_flight) {
     const int64_t n = s.tpr ? in_flight / ((s.tpr > 64 ? 1 : 256 / s.tpr) * s.chunks) : 1024;
     return n < 384 ? 256 : (n + 128) / 256 * 256;
@@ -768,9 +772,9 @@ int ln_bwd_blocks(int64_t rows, const Split& s) {
     return (int)(!s.tpr && n > rows ? rows : n > most ? most : n);
 }
 // Few rows (ln_bwd_few_kernel): one launch for two and no scratch, against reading x and dout twice and column sums that one workgroup makes
-// over all rows.  us of a call, two launches / one: 256 x 2048 fp32 8.4 / 5.3, 512 x 8192 bf16 12.4 / 10.8, 512 x 16384 fp32 32.0 / 28.1, 512 x
-// 8192 fp32 15.6 / 16.5; 1024 x 512 fp32 8.1 / 5.7, 1024 x 2048 bf16 9.0 / 10.0, 1000 x 4096 fp32 13.8 / 15.1 (and 2 us for the scratch's
-// allocation).
+// over all rows.  us on the device, two launches / one: 256 x 2048 fp32 7.4 / 4.5, 512 x 8192 bf16 14.9 / 11.0, 512 x 8192 fp32 16.5 / 17.1, 512 x
+// 16384 fp32 26.7 / 28.6; 1024 x 512 fp32 7.0 / 7.4, 1024 x 2048 bf16 10.2 / 12.5.  A call with its host time, the second launch and the
+// scratch's allocation among it: 16.4 / 11.8 for each of them but 512 x 8192 fp32, 16.5 / 16.6, and 512 x 16384, 26.3 / 28.1.
 bool ln_bwd_few(int dtype, int64_t rows, int cols) {
     return ln_few_split(dtype, cols).tpr && (rows <= 512 || (rows <= 1024 && rows * ln_chunks(dtype, cols) <= 1 << 18));
 }
